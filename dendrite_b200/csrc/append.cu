@@ -20,13 +20,6 @@
 
 namespace dd {
 
-__device__ __forceinline__ int floor_log2_pos(float a) {
-  const uint32_t b = __float_as_uint(a);
-  const int e = (int)((b >> 23) & 0xff);
-  if (e != 0) return e - 127;
-  return (31 - __clz((int)(b & 0x7fffff))) - 149;
-}
-
 // One warp per (token, K/V, head); lane owns E = D/32 consecutive elements.
 template <int D>
 __global__ void append_batch_kernel(int32_t n, int Hkv, int num_pages, int pool_dtype, int src_dtype,

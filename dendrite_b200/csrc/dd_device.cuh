@@ -73,6 +73,14 @@ __device__ __forceinline__ float e8m0_byte_to_float(uint32_t w, uint32_t b) {
   return e8m0_bits_to_float(__byte_perm(w, 0u, 0x0444u | (b << 12)) >> 1);
 }
 
+// floor(log2 a) of a positive f32, subnormals included.
+__device__ __forceinline__ int floor_log2_pos(float a) {
+  const uint32_t b = __float_as_uint(a);
+  const int e = (int)((b >> 23) & 0xff);
+  if (e != 0) return e - 127;
+  return (31 - __clz((int)(b & 0x7fffff))) - 149;
+}
+
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);

@@ -1,0 +1,99 @@
+// Shared pieces of the sliding-window attention kernels (window.cu,
+// window_mma.cu, window_tc.cu): arguments, the rows of a ragged batch and the
+// pages that a range of query positions sees.
+#pragma once
+#include "dd_device.cuh"
+
+namespace dd {
+
+struct WinArgs {
+  const void* q;       // [rows][Hq][D], q_stride elements from row to row
+  int64_t q_stride;
+  const void* kv;
+  const void* scales;
+  void* out;           // [rows][Hq][D] in q_dtype
+  float* lse;          // [rows][Hq], natural log, or NULL
+  uint32_t* status;    // 2 words, or NULL
+  const int32_t* row_indptr;   // NULL: one row per sequence
+  const int32_t* page_indptr;
+  const int32_t* page_indices;
+  const int32_t* num_tokens;
+  int32_t num_seqs, num_rows;
+  int32_t window, sinks;
+  int32_t Hq, Hkv, g, D, kv_dtype, q_dtype, gqa_map, num_pages;
+  float scale_log2;
+};
+
+// status: the first error's code and detail.
+__device__ __forceinline__ void win_report(uint32_t* status, uint32_t code, uint32_t aux) {
+  if (status && atomicCAS(status, 0u, code) == 0u) status[1] = aux;
+}
+
+// Rows [r0, r0 + m) of the batch belong to sequence s, whose row i has
+// position pos0 + i (negative: a row without a token, which sees nothing).
+// Row ranges are cut to the num_rows that the buffers hold.
+struct SeqRows {
+  int32_t r0, m, pos0, n;
+};
+__device__ __forceinline__ SeqRows seq_rows(const int32_t* row_indptr, const int32_t* num_tokens,
+                                            int32_t num_rows, int32_t s) {
+  SeqRows q;
+  q.n = max(num_tokens[s], 0);
+  int32_t a = s, b = s + 1;
+  if (row_indptr) {
+    a = row_indptr[s];
+    b = row_indptr[s + 1];
+  }
+  q.pos0 = q.n - (b - a);
+  q.r0 = min(max(a, 0), num_rows);
+  q.m = max(min(b, num_rows) - q.r0, 0);
+  return q;
+}
+
+// The sequence that owns a row: the last s with row_indptr[s] <= row (empty
+// sequences before it share its start), or -1 for a row behind the last one.
+__device__ __forceinline__ int32_t seq_of_row(const int32_t* row_indptr, int32_t num_seqs,
+                                              int32_t row) {
+  if (!row_indptr) return row < num_seqs ? row : -1;
+  if (num_seqs <= 0 || row < row_indptr[0] || row >= row_indptr[num_seqs]) return -1;
+  int32_t lo = 0, hi = num_seqs;  // row_indptr[lo] <= row < row_indptr[hi]
+  while (hi - lo > 1) {
+    const int32_t mid = (lo + hi) >> 1;
+    if (row_indptr[mid] <= row)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// The pages that hold a token visible to some position of [p_lo, p_hi], in
+// order: `ns` pages of first tokens, then the windows' pages from page `wp`.
+// Page v of the list is table entry page(v).
+struct WinPages {
+  int32_t ns, wp, count;
+  __device__ __forceinline__ int32_t page(int32_t v) const { return v < ns ? v : wp + v - ns; }
+};
+__device__ __forceinline__ WinPages win_pages(int32_t window, int32_t sinks, int32_t p_lo,
+                                              int32_t p_hi) {
+  WinPages w;
+  if (p_hi < 0) {
+    w.ns = w.wp = w.count = 0;
+    return w;
+  }
+  const int32_t first = window > 0 ? max(0, max(p_lo, 0) - window + 1) : 0;
+  w.wp = first / kPageSize;
+  w.ns = min((int32_t)(((int64_t)min(sinks, first) + kPageSize - 1) / kPageSize), w.wp);
+  w.count = w.ns + p_hi / kPageSize - w.wp + 1;
+  return w;
+}
+
+// Whether position p sees token j (p >= 0 or nothing).
+__device__ __forceinline__ bool win_sees(int32_t window, int32_t sinks, int32_t p, int32_t j) {
+  return j <= p && (window == 0 || j > p - window || j < sinks);
+}
+
+// Kernel launches (each returns a dd_status).
+int launch_win_simple(const WinArgs& a, cudaStream_t st);
+
+}  // namespace dd

@@ -299,6 +299,87 @@ int dd_decode_paged_static(const dd_attn_config* cfg, int32_t batch_size,
  * reference. */
 int dd_decode_paged_static_status(dd_stream_t stream, uint32_t* code, uint32_t* aux);
 
+/* Sliding-window attention over the paged cache ------------------------------
+ * For layers whose tokens attend to the last `window` tokens and to the first
+ * `sinks` ones. The reference only declares the field (`sliding_window`,
+ * crates/dendrite-core/src/attention/backend.rs:27,43-46) and never reads it.
+ *
+ * The batch is described by device arrays alone (no plan, no host copy of the
+ * tables), so a call can be captured into a CUDA graph and replayed while the
+ * arrays' contents change. Sequence s has num_tokens[s] tokens in the cache,
+ * the pages page_indices[page_indptr[s] .. page_indptr[s+1]); its last m tokens
+ * are the new ones, whose rows of q and out are
+ * q_indptr[s] .. q_indptr[s+1] (m of them; in the decode form row s, m = 1).
+ * The query of position p = num_tokens[s] - m + i sees the tokens
+ *   j <= p  with  j > p - window  or  j < sinks
+ * (window = 0: every j <= p; sinks then change nothing). A row that sees
+ * nothing (p < 0) gets zeros and LSE -inf.
+ *
+ * What is read: only pages that hold a visible token. The table entries of the
+ * others (pages that the engine gave back) are never looked at and may hold
+ * anything; so may slots at or past num_tokens[s]. A visible page whose id is
+ * outside the pool, or past the end of the sequence's table, is skipped, and
+ * if `status` (device, 2 x uint32, may be NULL; the caller clears it) is given,
+ * status[0] = 1 and status[1] = one such id (or the missing page's index);
+ * status[0] = 2: a bounded wait ran out and the outputs are not valid.
+ * Tokens that some new token of a sequence sees must be finite for all of
+ * that call's rows of the sequence to be: a row whose own window excludes
+ * them may still multiply them by a weight of zero.
+ *
+ * q: rows of [num_qo_heads][head_dim], q_stride elements from row to row
+ * (>= num_qo_heads * head_dim, a multiple of 16 bytes, so that the queries of
+ * a fused projection's output can be taken in place; 16-byte aligned).
+ * out: [rows][num_qo_heads][head_dim], dense, 16-byte aligned. lse as above
+ * (may be NULL). Rows at or past q_indptr[num_seqs] are left as they are.
+ * max_pages_per_seq (0: not known) only guides how the work is divided.
+ * No workspace; one kernel per call; calls on different streams are
+ * independent. bf16 queries over bf16 / E4M3 / MXFP8 pages run on the tensor
+ * cores; f32 queries or pages on the CUDA cores. */
+int dd_decode_paged_window(const dd_attn_config* cfg, int32_t batch_size,
+                           int32_t max_pages_per_seq, int32_t window, int32_t sinks,
+                           const void* q, int64_t q_stride, const void* kv_pages,
+                           const void* kv_scales, const int32_t* page_indptr,
+                           const int32_t* page_indices, const int32_t* num_tokens, void* out,
+                           float* lse, uint32_t* status, dd_stream_t stream);
+/* The chunk form: num_rows is the number of rows of q and out. */
+int dd_prefill_paged_window(const dd_attn_config* cfg, int32_t num_seqs, int32_t num_rows,
+                            int32_t max_pages_per_seq, int32_t window, int32_t sinks,
+                            const void* q, int64_t q_stride, const void* kv_pages,
+                            const void* kv_scales, const int32_t* q_indptr,
+                            const int32_t* page_indptr, const int32_t* page_indices,
+                            const int32_t* num_tokens, void* out, float* lse, uint32_t* status,
+                            dd_stream_t stream);
+
+/* Append of a ragged batch of new tokens into the sequences' pages, quantised
+ * as they are written (the codes dd_append_kv_batch and dd_quantize_kv_pages
+ * write). The batch is described as above: num_tokens[s] counts the new tokens
+ * already, and row new_indptr[s] + i of k, v holds token
+ * num_tokens[s] - m + i, m = new_indptr[s+1] - new_indptr[s] (new_indptr NULL:
+ * one row per sequence). k, v: rows of [num_kv_heads][head_dim] in src_dtype
+ * (F32 or BF16), k_stride / v_stride elements from row to row (multiples of 16
+ * bytes; 16-byte aligned). A token whose page is missing or outside the pool
+ * is skipped (status[0] = 1, status[1] = its row); rows at or past
+ * new_indptr[num_seqs] are not read. No two rows may go to one slot. */
+int dd_append_kv_paged(const dd_attn_config* cfg, void* kv_pages, void* kv_scales,
+                       int32_t num_seqs, int32_t num_rows, const int32_t* new_indptr,
+                       const int32_t* page_indptr, const int32_t* page_indices,
+                       const int32_t* num_tokens, const void* k, int64_t k_stride,
+                       const void* v, int64_t v_stride, int32_t src_dtype, uint32_t* status,
+                       dd_stream_t stream);
+
+/* Read-back: row out_indptr[s] + i of k_out, v_out ([rows][num_kv_heads]
+ * [head_dim], dense, 16-byte aligned, out_dtype F32 or BF16) becomes token
+ * first_token[s] + i of sequence s (first_token NULL: from token 0), for
+ * i < out_indptr[s+1] - out_indptr[s]: the stored value, code * scale for FP8
+ * pages, rounded once to out_dtype. A token whose page is missing or outside
+ * the pool reads as zeros (status[0] = 1, status[1] = its row); rows at or
+ * past out_indptr[num_seqs] are left as they are. The pool is not changed. */
+int dd_gather_kv_paged(const dd_attn_config* cfg, const void* kv_pages, const void* kv_scales,
+                       int32_t num_seqs, int32_t num_rows, const int32_t* out_indptr,
+                       const int32_t* first_token, const int32_t* page_indptr,
+                       const int32_t* page_indices, void* k_out, void* v_out, int32_t out_dtype,
+                       uint32_t* status, dd_stream_t stream);
+
 /* Merge of attention states: (o_a, lse_a) (+) (o_b, lse_b) -> (o, lse), f32,
  * natural-log LSE, element-wise over n rows of head_dim. The batched form of
  * merge_attention_outputs (crates/dendrite-ffi/src/flashinfer/cascade.rs:116-124).
