@@ -184,7 +184,8 @@ static int window_attention(const dd_attn_config* cfg, int32_t num_seqs, int32_t
   a.num_pages = cfg->num_pages;
   const float scale = cfg->scale > 0.f ? cfg->scale : 1.0f / std::sqrt((float)cfg->head_dim);
   a.scale_log2 = scale * kLog2e;
-  return launch_win_simple(a, st);
+  if (cfg->q_dtype == DD_DTYPE_F32 || cfg->kv_dtype == DD_DTYPE_F32) return launch_win_simple(a, st);
+  return launch_win_mma(a, max_pages, st);
 }
 
 }  // namespace dd

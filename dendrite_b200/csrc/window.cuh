@@ -95,5 +95,6 @@ __device__ __forceinline__ bool win_sees(int32_t window, int32_t sinks, int32_t 
 
 // Kernel launches (each returns a dd_status).
 int launch_win_simple(const WinArgs& a, cudaStream_t st);
+int launch_win_mma(const WinArgs& a, int max_pages, cudaStream_t st);
 
 }  // namespace dd

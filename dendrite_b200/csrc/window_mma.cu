@@ -1,0 +1,732 @@
+// Sliding-window attention for few query rows per sequence (decode, guessed
+// tokens): bf16 queries over bf16 / E4M3 / MXFP8 pages, head dims 64-256.
+//
+// Few rows read many tokens, so HBM bounds it: the kernel's work is to keep
+// loads in flight and to spend few instructions on each byte.
+//  - A warp takes one 16-token page at a time, straight from global memory
+//    into the fragment registers of its products: no shared memory, no
+//    barriers, every 32-byte sector read whole by one instruction. The
+//    products are transposed, S^T = K Q^T and O^T = V^T P^T (m16n8k16), so
+//    the page's tokens (and V's head dims) are the 16-row side and the 8-column
+//    side holds NT x 8 query rows: a GQA group of up to 8 wastes no second half.
+//    The head dims of K are contracted in an order in which a lane's share of
+//    a token is contiguous (Q is loaded in the same order); V's dims are dealt
+//    to the product's rows the same way, two tokens' words being interleaved
+//    with byte permutes.
+//  - K of the next page is requested as soon as S is formed, V of the next as
+//    soon as O is: half to all of a page is in flight for every warp.
+//  - S^T and O^T have their query row in the same lane, so the softmax state
+//    (reference, sum) and a rescale need no exchange; the reference moves only
+//    when a score passes it by 8 (log2 units), found by one vote a page.
+//  - FP8 codes are exact in f16, so FP8 pages take f16 products on the codes
+//    themselves: a row of Q is scaled by a power of two into f16's range, the
+//    per-head E4M3 scales are folded into the score scale and the epilogue,
+//    MXFP8's exponents of K scale S per 32-dim block, those of V scale the
+//    weights per block, relative to the largest exponent seen so far.
+//  - The warps of a CTA take pages in turn, the CTAs of a cluster (1 to 16)
+//    split the visible pages; the states are joined through shared memory and
+//    the cluster's shared memory, so a call is one launch without workspace.
+// Weights are rounded to two bf16 terms for bf16 pages (bf16's products take
+// both operands in bf16; two terms keep 16 bits) and to f16 for FP8 pages (11
+// bits, 2^-32 of the largest weight at worst); sums and references are f32.
+#include <algorithm>
+
+#include "window.cuh"
+
+namespace dd {
+
+constexpr int kWinWarps = 4;
+constexpr float kWinStep = 8.0f;     // how far a score may pass the reference (log2 units)
+constexpr float kWinF16Shift = 7.0f; // f16 weights are held as 2^7 w: below 2^16, normal down to 2^-21
+
+enum { kWinBf16 = 0, kWinE4m3 = 1, kWinMx = 2 };
+
+__device__ __forceinline__ uint4 ldg128(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg64(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ldg32(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t movm_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+template <bool kF16>
+__device__ __forceinline__ void win_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+  if (kF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two E4M3 codes (the low / high half of a word) as f16x2, exact.
+__device__ __forceinline__ uint32_t e4m3_f16(uint32_t codes, int hi) {
+  const __half2_raw h =
+      __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(hi ? codes >> 16 : codes & 0xffffu), __NV_E4M3);
+  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A page's K or V share of a lane, in the order of the products.
+//  K: token g + 8 * half, dims 32 i + 8 c .. + 8 (i < D / 32)
+//  V: bf16: token t(j), dims 64 i + 8 g .. + 8 (i < D / 64);
+//     FP8:  token t(j), dims 32 i + 4 g .. + 4 (i < D / 32);   t = 2c, 2c+1, 2c+8, 2c+9
+template <int D, int KV>
+struct WinFrag;
+template <int D>
+struct WinFrag<D, kWinBf16> {
+  uint4 k[D / 32][2];
+  uint4 v[D / 64][4];
+};
+template <int D, int KV>
+struct WinFrag {
+  uint2 k[D / 32][2];
+  uint32_t v[D / 32][4];
+  // MXFP8: exponent bytes of tokens g, g + 8 (D / 32 of them each)
+  uint32_t ek[2][(D + 127) / 128], ev[2][(D + 127) / 128];
+};
+
+template <int D>
+__device__ __forceinline__ void load_exps(const uint8_t* p, uint32_t (&e)[(D + 127) / 128]) {
+  if (D == 64) {
+    uint16_t x;
+    asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(x) : "l"(p));
+    e[0] = x;
+  } else if (D == 128) {
+    e[0] = ldg32(p);
+  } else {
+    const uint2 x = ldg64(p);
+    e[0] = x.x;
+    e[(D + 127) / 128 - 1] = x.y;
+  }
+}
+
+template <int D, int KV>
+__device__ __forceinline__ void load_k(WinFrag<D, KV>& f, const WinArgs& a, uint32_t page, int h, int g, int c) {
+  constexpr int kElem = KV == kWinBf16 ? 2 : 1;
+  const int64_t row = ((int64_t)page * 2 * a.Hkv + h) * kPageSize + g;
+  const uint8_t* p = reinterpret_cast<const uint8_t*>(a.kv) + (row * D + 8 * c) * kElem;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint8_t* q = p + (half * 8 * D + 32 * i) * kElem;
+      if constexpr (KV == kWinBf16)
+        f.k[i][half] = ldg128(q);
+      else
+        f.k[i][half] = ldg64(q);
+    }
+  if constexpr (KV == kWinMx) {
+    const uint8_t* e = reinterpret_cast<const uint8_t*>(a.scales) + row * (D / 32);
+    load_exps<D>(e, f.ek[0]);
+    load_exps<D>(e + 8 * (D / 32), f.ek[1]);
+  }
+}
+template <int D, int KV>
+__device__ __forceinline__ void load_v(WinFrag<D, KV>& f, const WinArgs& a, uint32_t page, int h, int g, int c) {
+  const int64_t slice = (((int64_t)page * 2 + 1) * a.Hkv + h) * kPageSize;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t row = slice + 2 * c + (j & 1) + 8 * (j >> 1);
+    if constexpr (KV == kWinBf16) {
+      const uint16_t* p = reinterpret_cast<const uint16_t*>(a.kv) + row * D + 8 * g;
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) f.v[i][j] = ldg128(p + 64 * i);
+    } else {
+      const uint8_t* p = reinterpret_cast<const uint8_t*>(a.kv) + row * D + 4 * g;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) f.v[i][j] = ldg32(p + 32 * i);
+    }
+  }
+  if constexpr (KV == kWinMx) {
+    const uint8_t* e = reinterpret_cast<const uint8_t*>(a.scales) + (slice + g) * (D / 32);
+    load_exps<D>(e, f.ev[0]);
+    load_exps<D>(e + 8 * (D / 32), f.ev[1]);
+  }
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+__device__ __forceinline__ uint32_t word(const uint2& v, int i) { return i == 0 ? v.x : v.y; }
+
+template <int D, int NT>
+struct WinShared {
+  float o[kWinWarps][NT * 8][D + 4];  // per warp: its output, normalised by its own sum
+  float m[kWinWarps][NT * 8], l[kWinWarps][NT * 8];
+  float cm[NT * 8], cl[NT * 8];       // the CTA's joined state (o[0] holds its output)
+};
+
+__device__ __forceinline__ float cluster_ld(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_ld4(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(r) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+// Tile t of the batch: sequence and tile within it. Sequence s owns the tiles
+// from s + floor(start(s) * g / R): at least the ceil(m * g / R) that it needs,
+// so no prefix sum over the sequences is wanted; surplus tiles have no rows.
+__device__ __forceinline__ void win_tile(const WinArgs& a, int R, int64_t t, int32_t& s, int32_t& tile) {
+  if (!a.row_indptr) {
+    const int per = (a.g + R - 1) / R;
+    s = (int32_t)(t / per);
+    tile = (int32_t)(t % per);
+    return;
+  }
+  int32_t lo = 0, hi = a.num_seqs;
+  auto base = [&](int32_t i) {
+    return i + (int64_t)min(max(a.row_indptr[i], 0), a.num_rows) * a.g / R;
+  };
+  while (hi - lo > 1) {
+    const int32_t mid = (lo + hi) >> 1;
+    if (base(mid) <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  s = lo;
+  tile = (int32_t)(t - base(lo));
+}
+
+template <int D, int KV, int NT>
+__global__ void __launch_bounds__(kWinWarps * 32, D * NT >= 256 ? 2 : 3) win_mma_kernel(WinArgs a, int nsplit) {
+  constexpr int R = NT * 8;
+  constexpr bool kF16 = KV != kWinBf16;
+  constexpr int kBlocks = D / 32;
+  __shared__ __align__(16) WinShared<D, NT> sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int rank = blockIdx.x % nsplit;
+  const int64_t unit = blockIdx.x / nsplit;
+  const int h = (int)(unit % a.Hkv);
+  int32_t s, tile;
+  win_tile(a, R, unit / a.Hkv, s, tile);
+  const SeqRows sr = seq_rows(a.row_indptr, a.num_tokens, a.num_rows, s);
+  const int64_t rows = (int64_t)sr.m * a.g, row0 = (int64_t)tile * R;
+  const int nrows = (int)min((int64_t)R, rows - row0);
+  if (nrows <= 0) return;  // the whole cluster
+  const int32_t p_lo = sr.pos0 + (int32_t)(row0 / a.g);
+  const int32_t p_hi = sr.pos0 + (int32_t)((row0 + nrows - 1) / a.g);
+  const WinPages wp = win_pages(a.window, a.sinks, p_lo, p_hi);
+  // This CTA's pages [v0, v1) of the visible ones; its warps take them in turn.
+  const int32_t v0 = (int32_t)((int64_t)rank * wp.count / nsplit), v1 = (int32_t)((int64_t)(rank + 1) * wp.count / nsplit);
+  const int32_t t0 = a.page_indptr[s], table = a.page_indptr[s + 1] - t0;
+
+  // Query row r of the tile -> its row of q and out.
+  auto q_row = [&](int r, int64_t& token) {
+    const int64_t rr = row0 + r;
+    token = sr.r0 + rr / a.g;
+    return qo_head_of(a.gqa_map, h, (int)(rr % a.g), a.Hkv, a.g);
+  };
+  // Page id of the lane's next page: one read for the warp's next 32.
+  int32_t base_v = v0 + warp;
+  auto read_ids = [&](int32_t v) {
+    const int32_t vv = v + kWinWarps * lane;
+    if (vv >= v1) return 0xFFFFFFFFu;
+    const int32_t idx = wp.page(vv);
+    const uint32_t id = idx < table ? (uint32_t)a.page_indices[t0 + idx] : 0xFFFFFFFFu;
+    if (id < (uint32_t)a.num_pages) return id;
+    win_report(a.status, kDevErrBadPage, idx < table ? id : (uint32_t)idx);
+    return 0xFFFFFFFFu;
+  };
+  uint32_t ids = read_ids(base_v);
+  int32_t at = 0;  // pages done of this read
+  uint32_t page = __shfl_sync(0xffffffffu, ids, 0);
+
+  WinFrag<D, KV> f;
+  if (page != 0xFFFFFFFFu) {
+    load_k<D, KV>(f, a, page, h, g, c);
+    load_v<D, KV>(f, a, page, h, g, c);
+  }
+
+  // Q fragments: lane (g, c) holds row 8 n + g, dims 32 i + 8 c .. + 8.
+  uint32_t q[NT][D / 32][4];
+  float scale[NT][2];   // score scale of columns 2c, 2c + 1
+  int32_t pos[NT][2];   // their positions
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int r = 8 * n + g;
+    int64_t token = 0;
+    const int hq = r < nrows ? q_row(r, token) : 0;
+    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) +
+                                                      token * a.q_stride + (int64_t)hq * D + 8 * c);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const uint4 x = r < nrows ? src[4 * i] : make_uint4(0, 0, 0, 0);
+      q[n][i][0] = x.x, q[n][i][1] = x.y, q[n][i][2] = x.z, q[n][i][3] = x.w;
+    }
+    float row_scale = a.scale_log2;
+    if (kF16) {
+      // The row times a power of two, its largest element just below 2^15:
+      // bf16's 8 bits then are exact in f16 down to 2^-29 of that element.
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = max(top, max(q[n][i][w] & 0x7fffu, (q[n][i][w] >> 16) & 0x7fffu));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int up = max(-126, min(127, 14 - ((int)(top >> 7) - 127)));
+      const float by = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          q[n][i][w] = pack_f16x2(__uint_as_float(q[n][i][w] << 16) * by,
+                                  __uint_as_float(q[n][i][w] & 0xffff0000u) * by);
+      // Two exact factors: 2^-up may be below f32's normal range by itself.
+      row_scale = row_scale * __uint_as_float((uint32_t)(127 - up / 2) << 23) *
+                  __uint_as_float((uint32_t)(127 - (up - up / 2)) << 23);
+      if (KV == kWinE4m3) row_scale *= reinterpret_cast<const float*>(a.scales)[h];
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      scale[n][e] = kF16 ? __shfl_sync(0xffffffffu, row_scale, (2 * c + e) * 4) : row_scale;
+      pos[n][e] = sr.pos0 + (int32_t)((row0 + 8 * n + 2 * c + e) / a.g);
+    }
+  }
+
+  float o[NT][D / 16][4];
+  float m[NT][2], l[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) m[n][e] = -INFINITY, l[n][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
+  }
+  uint32_t ref_e[(D + 127) / 128];  // MXFP8: largest exponent of V so far, per 32-dim block
+#pragma unroll
+  for (int i = 0; i < (D + 127) / 128; ++i) ref_e[i] = 0;
+
+  for (int32_t v = v0 + warp; v < v1; v += kWinWarps) {
+    // The next page's id, so its loads can go out as registers free up.
+    uint32_t next;
+    if (++at == 32) {
+      base_v = v + kWinWarps;
+      ids = read_ids(base_v);
+      at = 0;
+    }
+    next = __shfl_sync(0xffffffffu, ids, at);
+    if (v + kWinWarps >= v1) next = 0xFFFFFFFFu;
+    if (page == 0xFFFFFFFFu) {  // a bad page: skipped
+      page = next;
+      if (page != 0xFFFFFFFFu) {
+        load_k<D, KV>(f, a, page, h, g, c);
+        load_v<D, KV>(f, a, page, h, g, c);
+      }
+      continue;
+    }
+    // ---- S^T = K Q^T
+    float x[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[n][e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      if constexpr (KV == kWinBf16) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            win_mma<false>(x[n], word(f.k[i][0], 2 * u), word(f.k[i][1], 2 * u), word(f.k[i][0], 2 * u + 1),
+                           word(f.k[i][1], 2 * u + 1), q[n][i][2 * u], q[n][i][2 * u + 1]);
+      } else {
+        float y[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[n][e] = KV == kWinMx ? 0.f : x[n][e];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t k0 = word(f.k[i][0], u), k1 = word(f.k[i][1], u);
+          const uint32_t a0 = e4m3_f16(k0, 0), a1 = e4m3_f16(k1, 0), a2 = e4m3_f16(k0, 1), a3 = e4m3_f16(k1, 1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) win_mma<true>(y[n], a0, a1, a2, a3, q[n][i][2 * u], q[n][i][2 * u + 1]);
+        }
+        if constexpr (KV == kWinMx) {
+          const float e0 = e8m0_byte_to_float(f.ek[0][i / 4], i % 4), e1 = e8m0_byte_to_float(f.ek[1][i / 4], i % 4);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            x[n][0] = fmaf(y[n][0], e0, x[n][0]);
+            x[n][1] = fmaf(y[n][1], e0, x[n][1]);
+            x[n][2] = fmaf(y[n][2], e1, x[n][2]);
+            x[n][3] = fmaf(y[n][3], e1, x[n][3]);
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[n][e] = y[n][e];
+        }
+      }
+    }
+    page = next;
+    if (page != 0xFFFFFFFFu) load_k<D, KV>(f, a, page, h, g, c);
+    // ---- mask. Most pages are seen whole by every row.
+    const int32_t j0 = wp.page(v) * kPageSize;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[n][e] *= scale[n][e & 1];
+    const bool whole = j0 + kPageSize - 1 <= p_lo &&
+                       (a.window == 0 || j0 > p_hi - a.window || j0 + kPageSize <= a.sinks);
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!win_sees(a.window, a.sinks, pos[n][e & 1], j0 + g + 8 * (e >> 1))) x[n][e] = -INFINITY;
+      // Slots that no row of the tile sees may hold anything: their V (and
+      // exponents) become zero, as zero times NaN is not.
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int32_t t = j0 + 2 * c + (j & 1) + 8 * (j >> 1);
+        const bool seen = t <= p_hi && (a.window == 0 || t > p_lo - a.window || t < a.sinks);
+        if (!seen) {
+          if constexpr (KV == kWinBf16) {
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) f.v[i][j] = make_uint4(0, 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) f.v[i][j] = 0;
+          }
+        }
+      }
+      if constexpr (KV == kWinMx) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int32_t t = j0 + g + 8 * half;
+          const bool seen = t <= p_hi && (a.window == 0 || t > p_lo - a.window || t < a.sinks);
+          if (!seen) {
+#pragma unroll
+            for (int i = 0; i < (D + 127) / 128; ++i) f.ev[half][i] = 0;
+          }
+        }
+      }
+    }
+    // ---- references: moved for all rows once some score passes its own by
+    // more than kWinStep (the first page always).
+    bool over = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) over |= fmaxf(x[n][e], x[n][e + 2]) > m[n][e] + kWinStep;
+    if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float t = fmaxf(x[n][e], x[n][e + 2]);
+#pragma unroll
+          for (int b = 4; b < 32; b <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, b));
+          t = fmaxf(t, m[n][e]);
+          const float by = m[n][e] == t ? 1.f : exp2f(m[n][e] - t);
+          m[n][e] = t;
+          l[n][e] *= by;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            o[n][i][e] *= by;
+            o[n][i][e + 2] *= by;
+          }
+        }
+    }
+    if constexpr (KV == kWinMx) {
+      bool up = false;
+#pragma unroll
+      for (int i = 0; i < (D + 127) / 128; ++i)
+        up |= __vmaxu4(__vmaxu4(f.ev[0][i], f.ev[1][i]), ref_e[i]) != ref_e[i];
+      if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+        for (int i = 0; i < (D + 127) / 128; ++i) {
+          uint32_t t = __vmaxu4(f.ev[0][i], f.ev[1][i]);
+#pragma unroll
+          for (int b = 4; b < 32; b <<= 1) t = __vmaxu4(t, __shfl_xor_sync(0xffffffffu, t, b));
+          t = __vmaxu4(t, ref_e[i]);
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            if (4 * i + b < kBlocks) {
+              const int down = (int)((t >> (8 * b)) & 255) - (int)((ref_e[i] >> (8 * b)) & 255);
+              const float by = down > 126 ? 0.f : __uint_as_float((uint32_t)(127 - down) << 23);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  o[n][2 * (4 * i + b)][e] *= by;
+                  o[n][2 * (4 * i + b) + 1][e] *= by;
+                }
+            }
+          }
+          ref_e[i] = t;
+        }
+      }
+    }
+    // ---- weights
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float ref = (m[n][e] == -INFINITY ? 0.f : m[n][e]) - (kF16 ? kWinF16Shift : 0.f);
+        x[n][e] = fast_exp2(x[n][e] - ref);
+        x[n][e + 2] = fast_exp2(x[n][e + 2] - ref);
+        l[n][e] += x[n][e] + x[n][e + 2];
+      }
+    }
+    // ---- O^T += V^T P^T
+    if constexpr (KV == kWinBf16) {
+      uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t a_hi, a_lo;
+          split_bf16x2(x[n][2 * half], x[n][2 * half + 1], a_hi, a_lo);
+          hi[n][half] = movm_trans(a_hi);
+          lo[n][half] = movm_trans(a_lo);
+        }
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t w0 = word(f.v[i][0], u), w1 = word(f.v[i][1], u), w2 = word(f.v[i][2], u), w3 = word(f.v[i][3], u);
+          const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
+          const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            win_mma<false>(o[n][4 * i + u], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+            win_mma<false>(o[n][4 * i + u], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+          }
+        }
+    } else {
+      uint32_t b[NT][2];
+      if constexpr (KV == kWinE4m3) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) b[n][half] = movm_trans(pack_f16x2(x[n][2 * half], x[n][2 * half + 1]));
+      }
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {
+        if constexpr (KV == kWinMx) {
+          // The block's weights: w * 2^(e - reference); 255 is the NaN exponent.
+          const int top = (int)((ref_e[i / 4] >> (8 * (i % 4))) & 255);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int e = (int)((f.ev[half][i / 4] >> (8 * (i % 4))) & 255);
+            const float by = e == 255 ? __uint_as_float(0x7fc00000u)
+                                      : top - e > 126 ? 0.f : __uint_as_float((uint32_t)(127 + e - top) << 23);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              b[n][half] = movm_trans(pack_f16x2(x[n][2 * half] * by, x[n][2 * half + 1] * by));
+          }
+        }
+        const uint32_t l0 = __byte_perm(f.v[i][0], f.v[i][1], 0x5140), h0 = __byte_perm(f.v[i][0], f.v[i][1], 0x7362);
+        const uint32_t l1 = __byte_perm(f.v[i][2], f.v[i][3], 0x5140), h1 = __byte_perm(f.v[i][2], f.v[i][3], 0x7362);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint32_t w0 = u ? h0 : l0, w1 = u ? h1 : l1;
+          const uint32_t a0 = e4m3_f16(w0, 0), a1 = e4m3_f16(w0, 1), a2 = e4m3_f16(w1, 0), a3 = e4m3_f16(w1, 1);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) win_mma<true>(o[n][2 * i + u], a0, a1, a2, a3, b[n][0], b[n][1]);
+        }
+      }
+    }
+    if (page != 0xFFFFFFFFu) load_v<D, KV>(f, a, page, h, g, c);
+  }
+
+  // ---- the warp's state, normalised by its own sum
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float t = l[n][e];
+#pragma unroll
+      for (int b = 4; b < 32; b <<= 1) t += __shfl_xor_sync(0xffffffffu, t, b);
+      const int r = 8 * n + 2 * c + e;
+      float inv = t == 0.f ? 0.f : 1.f / t;
+      if (KV == kWinE4m3) inv *= reinterpret_cast<const float*>(a.scales)[a.Hkv + h];
+      if (g == 0) {
+        sh.m[warp][r] = m[n][e] - (kF16 ? kWinF16Shift : 0.f);
+        sh.l[warp][r] = t;
+      }
+      if constexpr (KV == kWinBf16) {
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          float4* dst = reinterpret_cast<float4*>(&sh.o[warp][r][64 * i + 8 * g]);
+          dst[0] = make_float4(o[n][4 * i][e] * inv, o[n][4 * i][e + 2] * inv, o[n][4 * i + 1][e] * inv, o[n][4 * i + 1][e + 2] * inv);
+          dst[1] = make_float4(o[n][4 * i + 2][e] * inv, o[n][4 * i + 2][e + 2] * inv, o[n][4 * i + 3][e] * inv, o[n][4 * i + 3][e + 2] * inv);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+          const float by = KV == kWinMx ? inv * e8m0_byte_to_float(ref_e[i / 4], i % 4) : inv;
+          *reinterpret_cast<float4*>(&sh.o[warp][r][32 * i + 4 * g]) =
+              make_float4(o[n][2 * i][e] * by, o[n][2 * i][e + 2] * by, o[n][2 * i + 1][e] * by, o[n][2 * i + 1][e + 2] * by);
+        }
+      }
+    }
+  __syncthreads();
+
+  // ---- join the warps (into o[0]), then the CTAs of the cluster
+  constexpr int kVec = D / 4;
+  auto weights = [](float mm, float ll, float top) { return ll * exp2f(mm - (top == -INFINITY ? 0.f : top)); };
+  for (int idx = threadIdx.x; idx < nrows * kVec; idx += kWinWarps * 32) {
+    const int r = idx / kVec, d = idx % kVec * 4;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWinWarps; ++w) top = fmaxf(top, sh.m[w][r]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWinWarps; ++w) {
+      const float wt = weights(sh.m[w][r], sh.l[w][r], top);
+      const float4 y = *reinterpret_cast<const float4*>(&sh.o[w][r][d]);
+      sum += wt;
+      acc.x = fmaf(wt, y.x, acc.x), acc.y = fmaf(wt, y.y, acc.y);
+      acc.z = fmaf(wt, y.z, acc.z), acc.w = fmaf(wt, y.w, acc.w);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<float4*>(&sh.o[0][r][d]) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    if (d == 0) {
+      sh.cm[r] = top;
+      sh.cl[r] = sum;
+    }
+  }
+  if (nsplit > 1)
+    cluster_barrier();
+  else
+    __syncthreads();
+  for (int idx = threadIdx.x + rank * kWinWarps * 32; idx < nrows * kVec; idx += nsplit * kWinWarps * 32) {
+    const int r = idx / kVec, d = idx % kVec * 4;
+    float top, sum;
+    float4 acc;
+    if (nsplit == 1) {
+      acc = *reinterpret_cast<const float4*>(&sh.o[0][r][d]);
+      top = sh.cm[r];
+      sum = sh.cl[r];
+    } else {
+      const uint32_t am = smem_u32(&sh.cm[r]), al = smem_u32(&sh.cl[r]), ao = smem_u32(&sh.o[0][r][d]);
+      top = -INFINITY;
+      sum = 0.f;
+      acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < nsplit; ++k) top = fmaxf(top, cluster_ld(am, k));
+      for (int k = 0; k < nsplit; ++k) {
+        const float wt = weights(cluster_ld(am, k), cluster_ld(al, k), top);
+        const float4 y = cluster_ld4(ao, k);
+        sum += wt;
+        acc.x = fmaf(wt, y.x, acc.x), acc.y = fmaf(wt, y.y, acc.y);
+        acc.z = fmaf(wt, y.z, acc.z), acc.w = fmaf(wt, y.w, acc.w);
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    }
+    int64_t token;
+    const int hq = q_row(r, token);
+    const int64_t dst = token * a.Hq + hq;
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + dst * D + d) =
+        make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+    if (d == 0 && a.lse) a.lse[dst] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  }
+  if (nsplit > 1) cluster_barrier();  // no CTA leaves while another reads its state
+}
+
+// ------------------------------------------------------------------ host side
+template <int D, int KV, int NT>
+static int launch_win_mma_t(const WinArgs& a, int64_t tiles, int nsplit, cudaStream_t st) {
+  const int64_t blocks = tiles * a.Hkv * nsplit;
+  if (blocks > 0x7FFFFFFF) return fail(DD_ERR_INVALID_ARGUMENT, "too many rows");
+  cudaError_t e = cudaSuccess;
+  if (nsplit > 8)
+    e = cudaFuncSetAttribute(win_mma_kernel<D, KV, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(kWinWarps * 32);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = nsplit;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = nsplit > 1 ? 1 : 0;
+    ProfScope ps(kProfMma, st);
+    e = cudaLaunchKernelEx(&cfg, win_mma_kernel<D, KV, NT>, a, nsplit);
+  }
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(DD_ERR_CUDA, std::string("window attention launch: ") + cudaGetErrorString(e));
+  return DD_OK;
+}
+
+template <int D, int KV>
+static int launch_win_mma_nt(const WinArgs& a, int nt, int64_t tiles, int nsplit, cudaStream_t st) {
+  if constexpr (D < 256)
+    if (nt == 2) return launch_win_mma_t<D, KV, 2>(a, tiles, nsplit, st);
+  return launch_win_mma_t<D, KV, 1>(a, tiles, nsplit, st);
+}
+template <int D>
+static int launch_win_mma_kv(const WinArgs& a, int nt, int64_t tiles, int nsplit, cudaStream_t st) {
+  switch (a.kv_dtype) {
+    case DD_DTYPE_BF16: return launch_win_mma_nt<D, kWinBf16>(a, nt, tiles, nsplit, st);
+    case DD_DTYPE_E4M3: return launch_win_mma_nt<D, kWinE4m3>(a, nt, tiles, nsplit, st);
+    default: return launch_win_mma_nt<D, kWinMx>(a, nt, tiles, nsplit, st);
+  }
+}
+
+// max_pages: pages of the longest table, 0 if not known.
+int launch_win_mma(const WinArgs& a, int max_pages, cudaStream_t st) {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  // Rows of an average sequence: one column block of 8 where they fit it, or
+  // where two of head_dim 256 would not fit the registers.
+  const int64_t rows = std::max<int64_t>(1, ((int64_t)a.num_rows * a.g + a.num_seqs - 1) / a.num_seqs);
+  const int nt = rows <= 8 || a.D == 256 ? 1 : 2, R = 8 * nt;
+  const int64_t tiles = a.row_indptr ? a.num_seqs + (int64_t)a.num_rows * a.g / R
+                                     : (int64_t)a.num_seqs * ((a.g + R - 1) / R);
+  // Cluster size: about four CTAs for each of the three that an SM holds, so
+  // that unequal sequences even out, but at least two pages for each warp.
+  int64_t pages = max_pages > 0 ? max_pages : INT64_MAX;
+  if (a.window > 0) pages = std::min(pages, ((int64_t)a.window + a.sinks) / kPageSize + 2);
+  const int64_t units = std::max<int64_t>(1, (a.row_indptr ? std::max<int64_t>(1, (int64_t)a.num_rows * a.g / R) : tiles) * a.Hkv);
+  const int64_t want = std::min<int64_t>((12 * (int64_t)sms + units - 1) / units, pages / (2 * kWinWarps));
+  int nsplit = 1;
+  while (nsplit < 16 && nsplit < want) nsplit *= 2;
+  switch (a.D) {
+    case 64: return launch_win_mma_kv<64>(a, nt, tiles, nsplit, st);
+    case 128: return launch_win_mma_kv<128>(a, nt, tiles, nsplit, st);
+    default: return launch_win_mma_kv<256>(a, nt, tiles, nsplit, st);
+  }
+}
+
+}  // namespace dd

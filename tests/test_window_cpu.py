@@ -175,7 +175,7 @@ def test_append_gather_refusals():
 @pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (7, 3), (40, 16)])
 def test_reference_against_a_loop(fmt, window, sinks):
     b = Batch(1, [5, 33, 0, 50], [5, 3, 2, 1], 4, 2, 64, fmt, False, window, sinks)
-    out, lse, _, _ = b.attention()
+    out, lse, _, _, _ = b.attention()
     vals, row = b.values(), 0
     for s, (n, m) in enumerate(zip(b.tokens, b.new)):
         for i in range(m):

@@ -109,13 +109,16 @@ class Batch:
 
     def attention(self, q=None, skip=lambda page: False):
         """(out, lse, size) of every row: size = sum_j w_j |v_j|, what a rounding
-        of the weights is relative to; and reach = max_j scale |q|.|k_j|."""
+        of the weights is relative to; reach = max_j scale |q|.|k_j|; and mass =
+        sum_j |v_j| (MXFP8: with the largest of the tokens' exponents in place
+        of each one's own), what weights that are tiny but not zero add up to."""
         vals = self.values()
         q = (self.q if q is None else q).double().numpy()
         out = np.zeros((self.rows, self.Hq, self.D))
         size = np.zeros_like(out)
         lse = np.full((self.rows, self.Hq), -np.inf)
         reach = np.zeros((self.rows, self.Hq))
+        mass = np.zeros_like(out)
         for s, (n, m) in enumerate(zip(self.tokens, self.new)):
             pos = np.arange(n - m, n)
             j = np.unique(np.concatenate([visible(p, self.window, self.sinks) for p in pos] or [[]])).astype(int)
@@ -143,7 +146,13 @@ class Batch:
                 dark = ~see.any(0)  # tokens that no row sees may hold anything
                 v = np.where(dark[:, None], 0, v)
                 out[r, h], size[r, h] = w @ v, w @ np.abs(v)
-        return out, lse, size, reach
+                av = np.abs(v)
+                if self.fmt == "mxfp8":
+                    e = self.scales.numpy()[page, 1, c, slot].astype(int)
+                    e = np.where(dark[:, None], 0, e)
+                    av *= np.repeat(2.0 ** (e.max(0) - e), 32, -1)
+                mass[r, h] = see @ np.where(dark[:, None], 0, av)
+        return out, lse, size, reach, mass
 
 
 def check_attention(got, got_lse, want, what="", weights=2.0 ** -8):
@@ -152,8 +161,12 @@ def check_attention(got, got_lse, want, what="", weights=2.0 ** -8):
     sum: 2^-18 covers them). A weight then is off by twice that, relatively, and
     by its rounding `weights` (half a step of the type that the products take);
     the sum adds D-independent f32 roundings (2^-16 covers sums of up to 2^8
-    terms per partial sum). The output is rounded once more."""
-    out, lse, size, reach = want
+    terms per partial sum). FP8 pages take f16 weights, held as 2^7 w relative
+    to a reference that is at most the largest weight: below f16's normal range
+    a weight is off by up to half of f16's smallest step, 2^-25 / 2^7 = 2^-32 of
+    the largest weight (which is at most 1), and times |v| these add up to
+    2^-32 mass. The output is rounded once more."""
+    out, lse, size, reach, mass = want
     got_t = got.dtype
     g, gl = got.detach().cpu().double().numpy(), got_lse.detach().cpu().double().numpy()
     dead = np.isinf(lse)
@@ -164,6 +177,6 @@ def check_attention(got, got_lse, want, what="", weights=2.0 ** -8):
     f = ~dead
     assert np.all(np.abs(gl - np.where(f, lse, 0))[f] <= (score + 2.0 ** -18 * (1 + np.abs(np.where(f, lse, 0))))[f]), f"{what}: lse"
     w = 2.0 ** -18 if got_t == torch.float32 else weights
-    tol = HALF[got_t] * np.abs(out) + (2 * score[..., None] + w + 2.0 ** -16) * size * (1 + HALF[got_t]) + 1e-30
+    tol = HALF[got_t] * np.abs(out) + (2 * score[..., None] + w + 2.0 ** -16) * size * (1 + HALF[got_t]) + 2.0 ** -32 * mass + 1e-30
     err = np.abs(g - out)
     assert np.all(err <= tol), f"{what}: worst error / bound {np.max(err / tol):.2f}"
