@@ -768,10 +768,11 @@ int make_kv_tensor_map(CUtensorMap* map, const void* kv, int64_t num_pages, int 
   } else {
     cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)D * elem_bytes};
-    cuuint32_t box[2] = {(cuuint32_t)(128 / elem_bytes), (cuuint32_t)kPageSize};
+    const bool narrow = D * elem_bytes < 128;  // rows of 64 FP8 codes: dense, unswizzled
+    cuuint32_t box[2] = {(cuuint32_t)(narrow ? D : 128 / elem_bytes), (cuuint32_t)kPageSize};
     cuuint32_t estr[2] = {1, 1};
     r = enc(map, dt, 2, const_cast<void*>(kv), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, narrow ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   }
   if (r != CUDA_SUCCESS) return fail(DD_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));

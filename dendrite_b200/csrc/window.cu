@@ -6,6 +6,7 @@
 // w_j = exp(x_j - lse), lse = log sum_j exp(x_j). The kernels walk the visible
 // pages once with a running maximum and sum (kept in f32, log2 domain); the
 // page table is read on the device, and no entry outside the visible pages.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -172,7 +173,7 @@ static int window_attention(const dd_attn_config* cfg, int32_t num_seqs, int32_t
   a.num_tokens = num_tokens;
   a.num_seqs = num_seqs;
   a.num_rows = num_rows;
-  a.window = window;
+  a.window = std::min(window, 1 << 30);  // no sequence is longer; keeps differences in 32 bits
   a.sinks = window > 0 ? sinks : 0;
   a.Hq = cfg->num_qo_heads;
   a.Hkv = cfg->num_kv_heads;
@@ -185,6 +186,10 @@ static int window_attention(const dd_attn_config* cfg, int32_t num_seqs, int32_t
   const float scale = cfg->scale > 0.f ? cfg->scale : 1.0f / std::sqrt((float)cfg->head_dim);
   a.scale_log2 = scale * kLog2e;
   if (cfg->q_dtype == DD_DTYPE_F32 || cfg->kv_dtype == DD_DTYPE_F32) return launch_win_simple(a, st);
+  // Rows of an average sequence; beyond 64 the wide tiles win.
+  const int64_t rows = (int64_t)num_rows * a.g / num_seqs;
+  const int64_t pool_rows = (int64_t)cfg->num_pages * 2 * a.Hkv * kPageSize;  // TMA coordinates are 32-bit
+  if (q_indptr && rows > 64 && a.D <= 128 && pool_rows > 0 && pool_rows <= 0x7FFFFFFF) return launch_win_tc(a, st);
   return launch_win_mma(a, max_pages, st);
 }
 

@@ -93,8 +93,60 @@ __device__ __forceinline__ bool win_sees(int32_t window, int32_t sinks, int32_t 
   return j <= p && (window == 0 || j > p - window || j < sinks);
 }
 
+// Two E4M3 codes (the low / high half of a word) as f16x2, exact.
+__device__ __forceinline__ uint32_t e4m3_f16(uint32_t codes, int hi) {
+  const __half2_raw h =
+      __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(hi ? codes >> 16 : codes & 0xffffu), __NV_E4M3);
+  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A bf16 query row as f16: the row times 2^up, its largest element (bf16 bits
+// `top`, sign off) just below 2^15. bf16's 8 bits then are exact down to 2^-29
+// of that element; what is smaller is off by at most 2^-39 of it.
+__device__ __forceinline__ int f16_row_shift(uint32_t top) {
+  return max(-126, min(127, 14 - ((int)(top >> 7) - 127)));
+}
+__device__ __forceinline__ uint32_t bf16x2_to_f16x2(uint32_t w, float by) {
+  return pack_f16x2(__uint_as_float(w << 16) * by, __uint_as_float(w & 0xffff0000u) * by);
+}
+// scale * 2^-up, in two exact steps (2^-up alone may be below f32's normal range).
+__device__ __forceinline__ float f16_score_scale(float scale, int up) {
+  return scale * __uint_as_float((uint32_t)(127 - up / 2) << 23) * __uint_as_float((uint32_t)(127 - (up - up / 2)) << 23);
+}
+
+// Tile t of the batch: sequence and tile within it. Sequence s owns the tiles
+// from s + floor(start(s) * g / R): at least the ceil(m * g / R) that it needs,
+// so no prefix sum over the sequences is wanted; surplus tiles have no rows,
+// and those before the first sequence's row come out as tile -1.
+__device__ __forceinline__ void win_tile(const WinArgs& a, int R, int64_t t, int32_t& s, int32_t& tile) {
+  if (!a.row_indptr) {
+    const int per = (a.g + R - 1) / R;
+    s = (int32_t)(t / per);
+    tile = (int32_t)(t % per);
+    return;
+  }
+  int32_t lo = 0, hi = a.num_seqs;
+  auto base = [&](int32_t i) {
+    return i + (int64_t)min(max(a.row_indptr[i], 0), a.num_rows) * a.g / R;
+  };
+  while (hi - lo > 1) {
+    const int32_t mid = (lo + hi) >> 1;
+    if (base(mid) <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  s = lo;
+  tile = (int32_t)max(t - base(lo), (int64_t)-1);
+}
+
 // Kernel launches (each returns a dd_status).
 int launch_win_simple(const WinArgs& a, cudaStream_t st);
 int launch_win_mma(const WinArgs& a, int max_pages, cudaStream_t st);
+int launch_win_tc(const WinArgs& a, cudaStream_t st);
 
 }  // namespace dd

@@ -76,17 +76,6 @@ __device__ __forceinline__ void win_mma(float (&c)[4], uint32_t a0, uint32_t a1,
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Two E4M3 codes (the low / high half of a word) as f16x2, exact.
-__device__ __forceinline__ uint32_t e4m3_f16(uint32_t codes, int hi) {
-  const __half2_raw h =
-      __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(hi ? codes >> 16 : codes & 0xffffu), __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
-}
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 // A page's K or V share of a lane, in the order of the products.
 //  K: token g + 8 * half, dims 32 i + 8 c .. + 8 (i < D / 32)
 //  V: bf16: token t(j), dims 64 i + 8 g .. + 8 (i < D / 64);
@@ -193,31 +182,6 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// Tile t of the batch: sequence and tile within it. Sequence s owns the tiles
-// from s + floor(start(s) * g / R): at least the ceil(m * g / R) that it needs,
-// so no prefix sum over the sequences is wanted; surplus tiles have no rows.
-__device__ __forceinline__ void win_tile(const WinArgs& a, int R, int64_t t, int32_t& s, int32_t& tile) {
-  if (!a.row_indptr) {
-    const int per = (a.g + R - 1) / R;
-    s = (int32_t)(t / per);
-    tile = (int32_t)(t % per);
-    return;
-  }
-  int32_t lo = 0, hi = a.num_seqs;
-  auto base = [&](int32_t i) {
-    return i + (int64_t)min(max(a.row_indptr[i], 0), a.num_rows) * a.g / R;
-  };
-  while (hi - lo > 1) {
-    const int32_t mid = (lo + hi) >> 1;
-    if (base(mid) <= t)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  s = lo;
-  tile = (int32_t)(t - base(lo));
-}
-
 template <int D, int KV, int NT>
 __global__ void __launch_bounds__(kWinWarps * 32, D * NT >= 256 ? 2 : 3) win_mma_kernel(WinArgs a, int nsplit) {
   constexpr int R = NT * 8;
@@ -233,7 +197,7 @@ __global__ void __launch_bounds__(kWinWarps * 32, D * NT >= 256 ? 2 : 3) win_mma
   const SeqRows sr = seq_rows(a.row_indptr, a.num_tokens, a.num_rows, s);
   const int64_t rows = (int64_t)sr.m * a.g, row0 = (int64_t)tile * R;
   const int nrows = (int)min((int64_t)R, rows - row0);
-  if (nrows <= 0) return;  // the whole cluster
+  if (tile < 0 || nrows <= 0) return;  // the whole cluster
   const int32_t p_lo = sr.pos0 + (int32_t)(row0 / a.g);
   const int32_t p_hi = sr.pos0 + (int32_t)((row0 + nrows - 1) / a.g);
   const WinPages wp = win_pages(a.window, a.sinks, p_lo, p_hi);
@@ -286,8 +250,6 @@ __global__ void __launch_bounds__(kWinWarps * 32, D * NT >= 256 ? 2 : 3) win_mma
     }
     float row_scale = a.scale_log2;
     if (kF16) {
-      // The row times a power of two, its largest element just below 2^15:
-      // bf16's 8 bits then are exact in f16 down to 2^-29 of that element.
       uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
@@ -295,17 +257,14 @@ __global__ void __launch_bounds__(kWinWarps * 32, D * NT >= 256 ? 2 : 3) win_mma
         for (int w = 0; w < 4; ++w) top = max(top, max(q[n][i][w] & 0x7fffu, (q[n][i][w] >> 16) & 0x7fffu));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int up = max(-126, min(127, 14 - ((int)(top >> 7) - 127)));
+      const int up = f16_row_shift(top);
       const float by = __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
       for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int w = 0; w < 4; ++w)
-          q[n][i][w] = pack_f16x2(__uint_as_float(q[n][i][w] << 16) * by,
-                                  __uint_as_float(q[n][i][w] & 0xffff0000u) * by);
-      // Two exact factors: 2^-up may be below f32's normal range by itself.
-      row_scale = row_scale * __uint_as_float((uint32_t)(127 - up / 2) << 23) *
-                  __uint_as_float((uint32_t)(127 - (up - up / 2)) << 23);
+          q[n][i][w] = bf16x2_to_f16x2(q[n][i][w], by);
+      row_scale = f16_score_scale(row_scale, up);
       if (KV == kWinE4m3) row_scale *= reinterpret_cast<const float*>(a.scales)[h];
     }
 #pragma unroll
