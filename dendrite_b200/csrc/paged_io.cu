@@ -18,6 +18,7 @@ struct PagedIo {
   const void* k;           // append: sources; gather: destinations
   const void* v;
   int64_t k_stride, v_stride;
+  int32_t log2_d;
 };
 
 // Page and slot of the token that a row stands for; false (and the status
@@ -45,102 +46,238 @@ __device__ __forceinline__ bool io_place(const PagedIo& a, int32_t row, bool rep
   return false;
 }
 
-// One warp per (row, K/V, head); lane owns E = D/32 consecutive elements.
-template <int D>
-__global__ void __launch_bounds__(256) append_paged_kernel(PagedIo a) {
-  constexpr int E = D / 32;
-  const int64_t w = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (w >= (int64_t)a.num_rows * 2 * a.Hkv) return;
-  const int32_t row = (int32_t)(w / (2 * a.Hkv));
-  const int rest = (int)(w % (2 * a.Hkv));
-  const int which = rest / a.Hkv, h = rest % a.Hkv;
-  uint32_t page;
-  int32_t slot;
-  bool live;
-  if (!io_place<true>(a, row, rest == 0 && lane == 0, page, slot, live)) return;
-  const int64_t src = (int64_t)row * (which ? a.v_stride : a.k_stride) + (int64_t)h * D + lane * E;
-  const void* from = which ? a.v : a.k;
-  float x[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    x[e] = a.ext_dtype == DD_DTYPE_F32 ? reinterpret_cast<const float*>(from)[src + e]
-                                       : bf16_bits_to_float(reinterpret_cast<const uint16_t*>(from)[src + e]);
-  const int64_t r = (((int64_t)page * 2 + which) * a.Hkv + h) * kPageSize + slot;
-  const int64_t dst = r * D + lane * E;
-  if (a.pool_dtype == DD_DTYPE_F32) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) reinterpret_cast<float*>(a.kv)[dst + e] = x[e];
-  } else if (a.pool_dtype == DD_DTYPE_BF16) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) reinterpret_cast<__nv_bfloat16*>(a.kv)[dst + e] = __float2bfloat16_rn(x[e]);
-  } else if (a.pool_dtype == DD_DTYPE_E4M3) {
-    const float sc = reinterpret_cast<const float*>(a.scales)[which * a.Hkv + h];
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      reinterpret_cast<uint8_t*>(a.kv)[dst + e] = float_to_e4m3_satrn(__fdiv_rn(x[e], sc));
-  } else {
-    float m = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) m = fmaxf(m, fabsf(x[e]));
-#pragma unroll
-    for (int o = 1; o < 32 / E; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const int ex = m > 0.f ? max(floor_log2_pos(m) - 8, -127) : -127;
-    const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);  // 2^-ex, a normal f32
-#pragma unroll
-    for (int e = 0; e < E; ++e) reinterpret_cast<uint8_t*>(a.kv)[dst + e] = float_to_e4m3_satrn(x[e] * inv);
-    if ((lane * E) % 32 == 0)
-      reinterpret_cast<uint8_t*>(a.scales)[r * (D / 32) + lane * E / 32] = (uint8_t)(ex + 127);
-  }
-}
+// A warp owns a row: its K and V heads are one run of 2 * Hkv * D elements, cut
+// into 16-byte chunks of the pool's type (kN elements). A lane takes every 32nd
+// chunk, four at a time with all their loads ahead of the work, so the row's
+// place in the page table (a short chain of dependent reads) is paid once for
+// up to 2 KB of codes. Pool-side accesses are whole 128-byte runs of one head.
+template <int POOL>
+struct IoPool {
+  static constexpr int kN = POOL == DD_DTYPE_F32 ? 4 : POOL == DD_DTYPE_BF16 ? 8 : 16;
+};
+constexpr int kIoWarps = 4;
+constexpr int kIoChunks = 4;  // chunks of a lane in flight
 
-template <int D>
-__global__ void __launch_bounds__(256) gather_paged_kernel(PagedIo a) {
-  constexpr int E = D / 32;
-  const int64_t w = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (w >= (int64_t)a.num_rows * 2 * a.Hkv) return;
-  const int32_t row = (int32_t)(w / (2 * a.Hkv));
-  const int rest = (int)(w % (2 * a.Hkv));
-  const int which = rest / a.Hkv, h = rest % a.Hkv;
-  uint32_t page;
-  int32_t slot;
-  bool live;
-  const bool ok = io_place<false>(a, row, rest == 0 && lane == 0, page, slot, live);
-  if (!live) return;
-  float x[E];
+// kN consecutive elements as f32, from / to 16-byte aligned (8 bytes for the
+// four bf16 of an f32 chunk) memory.
+template <int EXT, int N>
+__device__ __forceinline__ void io_load(const void* base, int64_t at, float (&x)[N]) {
+  if constexpr (EXT == DD_DTYPE_F32) {
+    const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(base) + at);
 #pragma unroll
-  for (int e = 0; e < E; ++e) x[e] = 0.f;
-  if (ok) {
-    const int64_t r = (((int64_t)page * 2 + which) * a.Hkv + h) * kPageSize + slot;
-    const int64_t src = r * D + lane * E;
-    if (a.pool_dtype == DD_DTYPE_F32) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = reinterpret_cast<const float*>(a.kv)[src + e];
-    } else if (a.pool_dtype == DD_DTYPE_BF16) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = bf16_bits_to_float(reinterpret_cast<const uint16_t*>(a.kv)[src + e]);
+    for (int i = 0; i < N / 4; ++i) {
+      const float4 v = p[i];
+      x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+    }
+  } else {
+    const uint2* p = reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(base) + at);
+    uint32_t w[N / 2];
+    if constexpr (N == 4) {
+      const uint2 v = *p;
+      w[0] = v.x, w[1] = v.y;
     } else {
-      const float s = a.pool_dtype == DD_DTYPE_E4M3
-                          ? reinterpret_cast<const float*>(a.scales)[which * a.Hkv + h]
-                          : e8m0_to_float(reinterpret_cast<const uint8_t*>(a.scales)[r * (D / 32) + lane * E / 32]);
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = e4m3_to_float(reinterpret_cast<const uint8_t*>(a.kv)[src + e]) * s;
+      for (int i = 0; i < N / 8; ++i) {
+        const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
-  void* to = const_cast<void*>(which ? a.v : a.k);
-  const int64_t dst = ((int64_t)row * a.Hkv + h) * D + lane * E;
+}
+template <int EXT, int N>
+__device__ __forceinline__ void io_store(void* base, int64_t at, const float (&x)[N]) {
+  if constexpr (EXT == DD_DTYPE_F32) {
+    float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(base) + at);
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    if (a.ext_dtype == DD_DTYPE_F32)
-      reinterpret_cast<float*>(to)[dst + e] = x[e];
-    else
-      reinterpret_cast<__nv_bfloat16*>(to)[dst + e] = __float2bfloat16_rn(x[e]);
+    for (int i = 0; i < N / 4; ++i) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+  } else {
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+    uint2* p = reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(base) + at);
+    if constexpr (N == 4) {
+      *p = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 8; ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
   }
 }
 
-static int io_check(const dd_attn_config* cfg, const void* kv, const void* scales, int32_t num_rows,
-                    const int32_t* page_indptr, const void* k, const void* v, int32_t ext_dtype) {
+// Chunk c of a row: K or V, head, element; pool row of that (page, K/V, head, slot).
+template <int N>
+struct IoChunk {
+  int which, h, d;
+  int64_t ext, row;
+  __device__ __forceinline__ IoChunk(const PagedIo& a, int c, int half, uint32_t page, int32_t slot) {
+    which = c >= half;
+    const int e = (which ? c - half : c) * N;
+    h = e >> a.log2_d;
+    d = e & ((1 << a.log2_d) - 1);
+    ext = e;
+    row = (((int64_t)page * 2 + which) * a.Hkv + h) * kPageSize + slot;
+  }
+};
+
+template <int POOL, int EXT>
+__global__ void __launch_bounds__(kIoWarps * 32) append_paged_kernel(PagedIo a) {
+  constexpr int N = IoPool<POOL>::kN;
+  const int64_t w = (int64_t)blockIdx.x * kIoWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (w >= a.num_rows) return;
+  const int32_t row = (int32_t)w;
+  uint32_t page;
+  int32_t slot;
+  bool live;
+  if (!io_place<true>(a, row, lane == 0, page, slot, live)) return;
+  const int half = (a.Hkv << a.log2_d) / N;
+  for (int c0 = lane; c0 - lane < 2 * half; c0 += 32 * kIoChunks) {
+    float x[kIoChunks][N];
+#pragma unroll
+    for (int u = 0; u < kIoChunks; ++u) {
+      const int c = c0 + 32 * u;
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[u][i] = 0.f;
+      if (c < 2 * half) {
+        const IoChunk<N> k(a, c, half, page, slot);
+        io_load<EXT, N>(k.which ? a.v : a.k, (int64_t)row * (k.which ? a.v_stride : a.k_stride) + k.ext, x[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kIoChunks; ++u) {
+      const int c = c0 + 32 * u;
+      const bool in = c < 2 * half;
+      const IoChunk<N> k(a, in ? c : 0, half, page, slot);
+      const int64_t dst = (k.row << a.log2_d) + k.d;
+      if constexpr (POOL == DD_DTYPE_F32 || POOL == DD_DTYPE_BF16) {
+        if (in) io_store<POOL, N>(a.kv, dst, x[u]);
+      } else {
+        if constexpr (POOL == DD_DTYPE_E4M3) {
+          const float sc = reinterpret_cast<const float*>(a.scales)[k.which * a.Hkv + k.h];
+#pragma unroll
+          for (int i = 0; i < N; ++i) x[u][i] = __fdiv_rn(x[u][i], sc);
+        } else {
+          // 32 elements are two neighbouring lanes' chunks.
+          float m = 0.f;
+#pragma unroll
+          for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[u][i]));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          const int ex = m > 0.f ? max(floor_log2_pos(m) - 8, -127) : -127;
+          const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);  // 2^-ex, a normal f32
+#pragma unroll
+          for (int i = 0; i < N; ++i) x[u][i] *= inv;
+          if (in && !(lane & 1))
+            reinterpret_cast<uint8_t*>(a.scales)[(k.row << (a.log2_d - 5)) + (k.d >> 5)] = (uint8_t)(ex + 127);
+        }
+        uint32_t q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          q[i] = e4m3x4_satrn(x[u][4 * i], x[u][4 * i + 1], x[u][4 * i + 2], x[u][4 * i + 3]);
+        if (in) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.kv) + dst) = make_uint4(q[0], q[1], q[2], q[3]);
+      }
+    }
+  }
+}
+
+template <int POOL, int EXT>
+__global__ void __launch_bounds__(kIoWarps * 32) gather_paged_kernel(PagedIo a) {
+  constexpr int N = IoPool<POOL>::kN;
+  const int64_t w = (int64_t)blockIdx.x * kIoWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (w >= a.num_rows) return;
+  const int32_t row = (int32_t)w;
+  uint32_t page;
+  int32_t slot;
+  bool live;
+  const bool ok = io_place<false>(a, row, lane == 0, page, slot, live);
+  if (!live) return;
+  const int half = (a.Hkv << a.log2_d) / N;
+  const int64_t width = (int64_t)a.Hkv << a.log2_d;
+  for (int c0 = lane; c0 < 2 * half; c0 += 32 * kIoChunks) {
+    uint4 v[kIoChunks];
+    float sc[kIoChunks];
+#pragma unroll
+    for (int u = 0; u < kIoChunks; ++u) {
+      const int c = c0 + 32 * u;
+      v[u] = make_uint4(0, 0, 0, 0);
+      sc[u] = 1.f;
+      if (ok && c < 2 * half) {
+        const IoChunk<N> k(a, c, half, page, slot);
+        v[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.kv) +
+                                               ((k.row << a.log2_d) + k.d) * (16 / N));
+        if constexpr (POOL == DD_DTYPE_E4M3) sc[u] = reinterpret_cast<const float*>(a.scales)[k.which * a.Hkv + k.h];
+        if constexpr (POOL == DD_DTYPE_MXFP8)
+          sc[u] = e8m0_to_float(reinterpret_cast<const uint8_t*>(a.scales)[(k.row << (a.log2_d - 5)) + (k.d >> 5)]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kIoChunks; ++u) {
+      const int c = c0 + 32 * u;
+      if (c >= 2 * half) break;
+      const IoChunk<N> k(a, c, half, 0, 0);
+      const uint32_t q[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+      float x[N];
+      if constexpr (POOL == DD_DTYPE_F32) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = __uint_as_float(q[i]);
+      } else if constexpr (POOL == DD_DTYPE_BF16) {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          x[2 * i] = __uint_as_float(q[i] << 16);
+          x[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          const float2 y = e4m3x2_to_float2((uint16_t)(i & 1 ? q[i / 2] >> 16 : q[i / 2] & 0xffffu));
+          x[2 * i] = y.x * sc[u];
+          x[2 * i + 1] = y.y * sc[u];
+        }
+      }
+      io_store<EXT, N>(const_cast<void*>(k.which ? a.v : a.k), (int64_t)row * width + k.ext, x);
+    }
+  }
+}
+
+template <int POOL>
+static void launch_io(bool append, const PagedIo& a, cudaStream_t st) {
+  const unsigned blocks = (unsigned)(((int64_t)a.num_rows + kIoWarps - 1) / kIoWarps);
+  ProfScope ps(kProfOther, st);
+  if (append) {
+    if (a.ext_dtype == DD_DTYPE_F32)
+      append_paged_kernel<POOL, DD_DTYPE_F32><<<blocks, kIoWarps * 32, 0, st>>>(a);
+    else
+      append_paged_kernel<POOL, DD_DTYPE_BF16><<<blocks, kIoWarps * 32, 0, st>>>(a);
+  } else {
+    if (a.ext_dtype == DD_DTYPE_F32)
+      gather_paged_kernel<POOL, DD_DTYPE_F32><<<blocks, kIoWarps * 32, 0, st>>>(a);
+    else
+      gather_paged_kernel<POOL, DD_DTYPE_BF16><<<blocks, kIoWarps * 32, 0, st>>>(a);
+  }
+}
+static int run_io(bool append, const PagedIo& a, cudaStream_t st) {
+  switch (a.pool_dtype) {
+    case DD_DTYPE_F32: launch_io<DD_DTYPE_F32>(append, a, st); break;
+    case DD_DTYPE_BF16: launch_io<DD_DTYPE_BF16>(append, a, st); break;
+    case DD_DTYPE_E4M3: launch_io<DD_DTYPE_E4M3>(append, a, st); break;
+    default: launch_io<DD_DTYPE_MXFP8>(append, a, st); break;
+  }
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess)
+    return fail(DD_ERR_CUDA, std::string(append ? "append_kv_paged" : "gather_kv_paged") + " launch: " + cudaGetErrorString(e));
+  return DD_OK;
+}
+
+static int log2_dim(int d) { return d == 64 ? 6 : d == 128 ? 7 : 8; }
+
+static int io_check(const dd_attn_config* cfg, const void* kv, const void* scales, const int32_t* page_indptr,
+                     const void* k, const void* v, int32_t ext_dtype) {
   if (!kv || !page_indptr || !k || !v) return fail(DD_ERR_INVALID_ARGUMENT, "NULL pointer");
   if (ext_dtype != DD_DTYPE_F32 && ext_dtype != DD_DTYPE_BF16)
     return fail(DD_ERR_INVALID_ARGUMENT, "K/V outside the pool must be f32 or bf16");
@@ -150,8 +287,6 @@ static int io_check(const dd_attn_config* cfg, const void* kv, const void* scale
     return fail(DD_ERR_INVALID_ARGUMENT, "kv_pages, k and v must be 16-byte aligned");
   if (fp8 && ((uintptr_t)scales & (cfg->kv_dtype == DD_DTYPE_MXFP8 ? 15 : 3)))
     return fail(DD_ERR_INVALID_ARGUMENT, "kv_scales not aligned");
-  if ((int64_t)num_rows * 2 * cfg->num_kv_heads / 8 >= 0x7FFFFFFF)
-    return fail(DD_ERR_INVALID_ARGUMENT, "too many rows");
   return DD_OK;
 }
 
@@ -172,7 +307,7 @@ extern "C" int dd_append_kv_paged(const dd_attn_config* cfg, void* kv_pages, voi
   if (!new_indptr && num_rows != num_seqs)
     return fail(DD_ERR_INVALID_ARGUMENT, "without new_indptr there is one row per sequence");
   if (!num_tokens) return fail(DD_ERR_INVALID_ARGUMENT, "num_tokens is NULL");
-  rc = io_check(cfg, kv_pages, kv_scales, num_rows, page_indptr, k, v, src_dtype);
+  rc = io_check(cfg, kv_pages, kv_scales, page_indptr, k, v, src_dtype);
   if (rc) return rc;
   const int64_t width = (int64_t)cfg->num_kv_heads * cfg->head_dim;
   const int elem = src_dtype == DD_DTYPE_F32 ? 4 : 2;
@@ -181,20 +316,8 @@ extern "C" int dd_append_kv_paged(const dd_attn_config* cfg, void* kv_pages, voi
                 "k_stride and v_stride must cover a row's heads and be multiples of 16 bytes");
   const PagedIo a{kv_pages, kv_scales, new_indptr, page_indptr, page_indices, num_tokens, status,
                   num_seqs, num_rows, cfg->num_kv_heads, cfg->num_pages, cfg->kv_dtype, src_dtype,
-                  k, v, k_stride, v_stride};
-  const unsigned blocks = (unsigned)(((int64_t)num_rows * 2 * cfg->num_kv_heads + 7) / 8);
-  cudaStream_t st = (cudaStream_t)stream;
-  {
-    ProfScope ps(kProfOther, st);
-    switch (cfg->head_dim) {
-      case 64: append_paged_kernel<64><<<blocks, 256, 0, st>>>(a); break;
-      case 128: append_paged_kernel<128><<<blocks, 256, 0, st>>>(a); break;
-      default: append_paged_kernel<256><<<blocks, 256, 0, st>>>(a); break;
-    }
-  }
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(DD_ERR_CUDA, std::string("append_kv_paged launch: ") + cudaGetErrorString(e));
-  return DD_OK;
+                  k, v, k_stride, v_stride, log2_dim(cfg->head_dim)};
+  return run_io(true, a, (cudaStream_t)stream);
 }
 
 extern "C" int dd_gather_kv_paged(const dd_attn_config* cfg, const void* kv_pages,
@@ -208,22 +331,10 @@ extern "C" int dd_gather_kv_paged(const dd_attn_config* cfg, const void* kv_page
   if (num_seqs < 0 || num_rows < 0) return fail(DD_ERR_INVALID_ARGUMENT, "num_seqs and num_rows must be >= 0");
   if (num_seqs == 0 || num_rows == 0) return DD_OK;
   if (!out_indptr) return fail(DD_ERR_INVALID_ARGUMENT, "out_indptr is NULL");
-  rc = io_check(cfg, kv_pages, kv_scales, num_rows, page_indptr, k_out, v_out, out_dtype);
+  rc = io_check(cfg, kv_pages, kv_scales, page_indptr, k_out, v_out, out_dtype);
   if (rc) return rc;
   const PagedIo a{const_cast<void*>(kv_pages), const_cast<void*>(kv_scales), out_indptr, page_indptr,
                   page_indices, first_token, status, num_seqs, num_rows, cfg->num_kv_heads,
-                  cfg->num_pages, cfg->kv_dtype, out_dtype, k_out, v_out, 0, 0};
-  const unsigned blocks = (unsigned)(((int64_t)num_rows * 2 * cfg->num_kv_heads + 7) / 8);
-  cudaStream_t st = (cudaStream_t)stream;
-  {
-    ProfScope ps(kProfOther, st);
-    switch (cfg->head_dim) {
-      case 64: gather_paged_kernel<64><<<blocks, 256, 0, st>>>(a); break;
-      case 128: gather_paged_kernel<128><<<blocks, 256, 0, st>>>(a); break;
-      default: gather_paged_kernel<256><<<blocks, 256, 0, st>>>(a); break;
-    }
-  }
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(DD_ERR_CUDA, std::string("gather_kv_paged launch: ") + cudaGetErrorString(e));
-  return DD_OK;
+                  cfg->num_pages, cfg->kv_dtype, out_dtype, k_out, v_out, 0, 0, log2_dim(cfg->head_dim)};
+  return run_io(false, a, (cudaStream_t)stream);
 }

@@ -182,8 +182,14 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
 }
 
+// CTAs an SM holds: FP8 pages are half the bytes of bf16 ones, so it takes more
+// warps to have as many in flight (128 x 2048 tokens of E4M3 / SM at 3 CTAs:
+// 131 us, 4: see the launch rule), as far as the registers go without spills.
 template <int D, int KV, int NT>
-__global__ void __launch_bounds__(kWinWarps * 32, D * NT >= 256 ? 2 : 3) win_mma_kernel(WinArgs a, int nsplit) {
+constexpr int kWinCtas = D * NT >= 256 ? 2 : KV != kWinBf16 || D == 64 ? 4 : 3;
+
+template <int D, int KV, int NT>
+__global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_kernel(WinArgs a, int nsplit) {
   constexpr int R = NT * 8;
   constexpr bool kF16 = KV != kWinBf16;
   constexpr int kBlocks = D / 32;

@@ -31,42 +31,41 @@ def _fail(msg: str):
 
 
 def _check_pool(cfg: AttnConfig, kv_pages, kv_scales) -> None:
-    if kv_pages.dtype not in _POOL.get(cfg.kv_dtype, ()) or not kv_pages.is_contiguous() or \
+    kvd = cfg.kv_dtype
+    if kv_pages.dtype not in _POOL.get(kvd, ()) or not kv_pages.is_contiguous() or \
             kv_pages.shape != (cfg.num_pages, 2, cfg.num_kv_heads, cfg.page_size, cfg.head_dim):
         _fail("kv_pages must be a dense [num_pages][2][Hkv][16][D] pool of the config's kv_dtype")
-    if cfg.kv_dtype == DTYPE_E4M3:
+    if kvd == DTYPE_E4M3:
         if kv_scales is None or kv_scales.dtype != torch.float32 or not kv_scales.is_contiguous() or \
                 kv_scales.numel() != 2 * cfg.num_kv_heads:
             _fail("E4M3 pages need dense f32 kv_scales [2][Hkv]")
-    elif cfg.kv_dtype == DTYPE_MXFP8:
+    elif kvd == DTYPE_MXFP8:
         if kv_scales is None or kv_scales.dtype != torch.uint8 or not kv_scales.is_contiguous() or \
                 kv_scales.numel() * 32 != kv_pages.numel():
             _fail("MXFP8 pages need dense uint8 kv_scales [num_pages][2][Hkv][16][D/32]")
 
 
 def _check_index(name: str, t, n: int) -> None:
-    if t.dtype not in _INDEX or t.dim() != 1 or not t.is_contiguous() or t.numel() < n:
+    if t.dtype not in _INDEX or not t.is_contiguous() or t.dim() != 1 or t.numel() < n:
         _fail(f"{name} must be a dense int32 vector of at least {n}")
 
 
-def _check_rows(name: str, t, heads: int, dim: int) -> None:
-    """[rows][heads][dim], the heads dense behind one another, any row stride."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim or t.stride(2) != 1 or \
-            (heads > 1 and t.stride(1) != dim):
+def _check_rows(name: str, t, heads: int, dim: int) -> int:
+    """[rows][heads][dim], the heads dense behind one another, any row stride.
+    Returns the row stride; that of a single row may be anything and is not used."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim or stride[2] != 1 or \
+            (heads > 1 and stride[1] != dim):
         _fail(f"{name} must be [rows][{heads}][{dim}] with dense rows")
+    return stride[0] if shape[0] > 1 else max(stride[0], heads * dim)
 
 
-def _row_stride(t) -> int:
-    """Row stride in elements; that of a single row may be anything and is not used."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1] * t.shape[2])
-
-
-def _device(*tensors) -> torch.device:
-    dev = tensors[0].device
+def _device(*tensors) -> int:
+    dev = tensors[0].get_device()  # -1 on the host
     for t in tensors:
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != dev:
             _fail("all tensors must be on one device")
-    if dev.type != "cuda":
+    if dev < 0:
         _fail("the tensors must be on a CUDA device")
     return dev
 
@@ -79,20 +78,20 @@ def _status_ptr(status):
     return status.data_ptr()
 
 
-def _call(dev: torch.device, fn, name: str, args, stream) -> None:
+def _call(dev: int, fn, name: str, args, stream) -> None:
     """The C call with the tensors' device current, on `stream` or that device's current one."""
-    if stream is None:
-        stream = torch.cuda.current_stream(dev)
-    if torch.cuda.current_device() == dev.index:
-        check(fn(*args, stream.cuda_stream), name)
+    handle = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+    if torch.cuda.current_device() == dev:
+        check(fn(*args, handle), name)
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, stream.cuda_stream), name)
+            check(fn(*args, handle), name)
 
 
 def _attend(cfg, q, kv_pages, q_indptr, page_indptr, page_indices, num_tokens, window, sinks, max_pages,
             kv_scales, out, lse, status, stream):
-    _check_rows("q", q, cfg.num_qo_heads, cfg.head_dim)
+    heads, dim = cfg.num_qo_heads, cfg.head_dim
+    stride = _check_rows("q", q, heads, dim)
     if q.dtype != (torch.float32 if cfg.q_dtype == DTYPE_F32 else torch.bfloat16):
         _fail("q does not have the config's q_dtype")
     _check_pool(cfg, kv_pages, kv_scales)
@@ -105,7 +104,7 @@ def _attend(cfg, q, kv_pages, q_indptr, page_indptr, page_indices, num_tokens, w
     _check_index("page_indptr", page_indptr, seqs + 1)
     _check_index("page_indices", page_indices, 0)
     _check_index("num_tokens", num_tokens, seqs)
-    shape = (rows, cfg.num_qo_heads, cfg.head_dim)
+    shape = (rows, heads, dim)
     if out is not None and (out.dtype != q.dtype or out.shape != shape or not out.is_contiguous()):
         _fail("out must be dense, of q's shape and type")
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != shape[:2] or not lse.is_contiguous()):
@@ -113,12 +112,12 @@ def _attend(cfg, q, kv_pages, q_indptr, page_indptr, page_indices, num_tokens, w
     st = _status_ptr(status)
     dev = _device(q, kv_pages, kv_scales, q_indptr, page_indptr, page_indices, num_tokens, out, lse, status)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=dev)
+        out = q.new_empty(shape)
     if lse is None:
-        lse = torch.empty(shape[:2], dtype=torch.float32, device=dev)
+        lse = q.new_empty(shape[:2], dtype=torch.float32)
     head = (C.byref(cfg), seqs) if q_indptr is None else (C.byref(cfg), seqs, rows)
     tables = (page_indptr.data_ptr(), page_indices.data_ptr(), num_tokens.data_ptr())
-    args = head + (max_pages, window, sinks, q.data_ptr(), _row_stride(q), kv_pages.data_ptr(),
+    args = head + (max_pages, window, sinks, q.data_ptr(), stride, kv_pages.data_ptr(),
                    None if kv_scales is None else kv_scales.data_ptr())
     if q_indptr is None:
         _call(dev, lib.dd_decode_paged_window, "dd_decode_paged_window",
@@ -164,8 +163,8 @@ def append_kv_paged(cfg: AttnConfig, kv_pages: torch.Tensor, kv_scales: torch.Te
     f32, any row stride) as the last tokens of sequence s, quantising for FP8
     pools. num_tokens counts them already; new_indptr None: one per sequence."""
     _check_pool(cfg, kv_pages, kv_scales)
-    _check_rows("k", k, cfg.num_kv_heads, cfg.head_dim)
-    _check_rows("v", v, cfg.num_kv_heads, cfg.head_dim)
+    k_stride = _check_rows("k", k, cfg.num_kv_heads, cfg.head_dim)
+    v_stride = _check_rows("v", v, cfg.num_kv_heads, cfg.head_dim)
     if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float32) or k.shape[0] != v.shape[0]:
         _fail("k and v must both be bf16 or f32, of as many rows")
     rows = k.shape[0]
@@ -182,7 +181,7 @@ def append_kv_paged(cfg: AttnConfig, kv_pages: torch.Tensor, kv_scales: torch.Te
     _call(dev, lib.dd_append_kv_paged, "dd_append_kv_paged",
           (C.byref(cfg), kv_pages.data_ptr(), None if kv_scales is None else kv_scales.data_ptr(), seqs, rows,
            None if new_indptr is None else new_indptr.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(),
-           num_tokens.data_ptr(), k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v),
+           num_tokens.data_ptr(), k.data_ptr(), k_stride, v.data_ptr(), v_stride,
            DTYPE_F32 if k.dtype == torch.float32 else DTYPE_BF16, st), stream)
 
 
@@ -212,9 +211,9 @@ def gather_kv_paged(cfg: AttnConfig, kv_pages: torch.Tensor, kv_scales: torch.Te
     st = _status_ptr(status)
     dev = _device(kv_pages, kv_scales, out_indptr, first_token, page_indptr, page_indices, k, v, status)
     if k is None:
-        k = torch.empty(shape, dtype=out_dtype, device=dev)
+        k = kv_pages.new_empty(shape, dtype=out_dtype)
     if v is None:
-        v = torch.empty(shape, dtype=out_dtype, device=dev)
+        v = kv_pages.new_empty(shape, dtype=out_dtype)
     _call(dev, lib.dd_gather_kv_paged, "dd_gather_kv_paged",
           (C.byref(cfg), kv_pages.data_ptr(), None if kv_scales is None else kv_scales.data_ptr(), seqs, num_rows,
            out_indptr.data_ptr(), None if first_token is None else first_token.data_ptr(), page_indptr.data_ptr(),
