@@ -779,6 +779,28 @@ int make_kv_tensor_map(CUtensorMap* map, const void* kv, int64_t num_pages, int 
   return DD_OK;
 }
 
+// View of query rows [rows][Hq][D] (row_stride elements apart) as (64 dims, two
+// head axes, tokens) so that one box {64, group, 1, tokens} (grouped heads) or
+// {64, 1, group, tokens} (tiled) lands as [token][head of the group][128 B],
+// 128-byte swizzle. Rows past the last are zeros.
+int make_q_tensor_map(CUtensorMap* map, const void* q, int64_t rows, int64_t row_stride, int Hq, int Hkv, int D,
+                      int gqa_map, int tokens) {
+  PFN_encodeTiled enc = get_encode_fn();
+  if (!enc) return fail(DD_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const int g = Hq / Hkv;
+  const bool tiled = gqa_map == DD_GQA_TILED;
+  const int inner = tiled ? Hkv : g, outer = tiled ? g : Hkv;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)inner, (cuuint64_t)outer, (cuuint64_t)rows};
+  cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)inner * D * 2, (cuuint64_t)row_stride * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)(tiled ? 1 : g), (cuuint32_t)(tiled ? g : 1), (cuuint32_t)tokens};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(q), dims, strides, box, estr,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DD_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+  return DD_OK;
+}
+
 template <int D, int KV>
 static cudaError_t launch_mma_t(const CUtensorMap& map, const AttnArgs& a, cudaStream_t st,
                                bool after_tc) {

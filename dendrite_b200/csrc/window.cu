@@ -188,8 +188,7 @@ static int window_attention(const dd_attn_config* cfg, int32_t num_seqs, int32_t
   if (cfg->q_dtype == DD_DTYPE_F32 || cfg->kv_dtype == DD_DTYPE_F32) return launch_win_simple(a, st);
   // Rows of an average sequence; beyond 64 the wide tiles win.
   const int64_t rows = (int64_t)num_rows * a.g / num_seqs;
-  const int64_t pool_rows = (int64_t)cfg->num_pages * 2 * a.Hkv * kPageSize;  // TMA coordinates are 32-bit
-  if (q_indptr && rows > 64 && a.D <= 128 && pool_rows > 0 && pool_rows <= 0x7FFFFFFF) return launch_win_tc(a, st);
+  if (q_indptr && rows > 64 && win_tc_fits(a)) return launch_win_tc(a, st);
   return launch_win_mma(a, max_pages, st);
 }
 

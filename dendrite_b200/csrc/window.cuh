@@ -93,11 +93,11 @@ __device__ __forceinline__ bool win_sees(int32_t window, int32_t sinks, int32_t 
   return j <= p && (window == 0 || j > p - window || j < sinks);
 }
 
-// Two E4M3 codes (the low / high half of a word) as f16x2, exact.
-__device__ __forceinline__ uint32_t e4m3_f16(uint32_t codes, int hi) {
-  const __half2_raw h =
-      __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(hi ? codes >> 16 : codes & 0xffffu), __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// Four E4M3 codes (a word) as two f16x2, exact: bytes 0-1 -> lo, 2-3 -> hi.
+__device__ __forceinline__ void e4m3x4_f16(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n .reg .b16 a, b;\n mov.b32 {a, b}, %2;\n cvt.rn.f16x2.e4m3x2 %0, a;\n cvt.rn.f16x2.e4m3x2 %1, b;\n}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(codes));
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -118,21 +118,20 @@ __device__ __forceinline__ float f16_score_scale(float scale, int up) {
   return scale * __uint_as_float((uint32_t)(127 - up / 2) << 23) * __uint_as_float((uint32_t)(127 - (up - up / 2)) << 23);
 }
 
-// Tile t of the batch: sequence and tile within it. Sequence s owns the tiles
-// from s + floor(start(s) * g / R): at least the ceil(m * g / R) that it needs,
-// so no prefix sum over the sequences is wanted; surplus tiles have no rows,
-// and those before the first sequence's row come out as tile -1.
-__device__ __forceinline__ void win_tile(const WinArgs& a, int R, int64_t t, int32_t& s, int32_t& tile) {
+// Tile t of the batch: sequence and tile within it, a tile being R of the
+// sequence's m * g rows. Sequence s owns the tiles from s + floor(start(s) * g
+// / R): at least the ceil(m * g / R) that it needs, so no prefix sum over the
+// sequences is wanted; surplus tiles have no rows, and those before the first
+// sequence's row come out as tile -1.
+__device__ __forceinline__ void win_tile(const WinArgs& a, int g, int R, int64_t t, int32_t& s, int32_t& tile) {
   if (!a.row_indptr) {
-    const int per = (a.g + R - 1) / R;
+    const int per = (g + R - 1) / R;
     s = (int32_t)(t / per);
     tile = (int32_t)(t % per);
     return;
   }
   int32_t lo = 0, hi = a.num_seqs;
-  auto base = [&](int32_t i) {
-    return i + (int64_t)min(max(a.row_indptr[i], 0), a.num_rows) * a.g / R;
-  };
+  auto base = [&](int32_t i) { return i + (int64_t)min(max(a.row_indptr[i], 0), a.num_rows) * g / R; };
   while (hi - lo > 1) {
     const int32_t mid = (lo + hi) >> 1;
     if (base(mid) <= t)
@@ -147,6 +146,7 @@ __device__ __forceinline__ void win_tile(const WinArgs& a, int R, int64_t t, int
 // Kernel launches (each returns a dd_status).
 int launch_win_simple(const WinArgs& a, cudaStream_t st);
 int launch_win_mma(const WinArgs& a, int max_pages, cudaStream_t st);
+bool win_tc_fits(const WinArgs& a);
 int launch_win_tc(const WinArgs& a, cudaStream_t st);
 
 }  // namespace dd

@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
   const int64_t unit = blockIdx.x / nsplit;
   const int h = (int)(unit % a.Hkv);
   int32_t s, tile;
-  win_tile(a, R, unit / a.Hkv, s, tile);
+  win_tile(a, a.g, R, unit / a.Hkv, s, tile);
   const SeqRows sr = seq_rows(a.row_indptr, a.num_tokens, a.num_rows, s);
   const int64_t rows = (int64_t)sr.m * a.g, row0 = (int64_t)tile * R;
   const int nrows = (int)min((int64_t)R, rows - row0);
@@ -336,8 +336,9 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
           for (int e = 0; e < 4; ++e) y[n][e] = KV == kWinMx ? 0.f : x[n][e];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const uint32_t k0 = word(f.k[i][0], u), k1 = word(f.k[i][1], u);
-          const uint32_t a0 = e4m3_f16(k0, 0), a1 = e4m3_f16(k1, 0), a2 = e4m3_f16(k0, 1), a3 = e4m3_f16(k1, 1);
+          uint32_t a0, a1, a2, a3;
+          e4m3x4_f16(word(f.k[i][0], u), a0, a2);
+          e4m3x4_f16(word(f.k[i][1], u), a1, a3);
 #pragma unroll
           for (int n = 0; n < NT; ++n) win_mma<true>(y[n], a0, a1, a2, a3, q[n][i][2 * u], q[n][i][2 * u + 1]);
         }
@@ -521,8 +522,9 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
         const uint32_t l1 = __byte_perm(f.v[i][2], f.v[i][3], 0x5140), h1 = __byte_perm(f.v[i][2], f.v[i][3], 0x7362);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const uint32_t w0 = u ? h0 : l0, w1 = u ? h1 : l1;
-          const uint32_t a0 = e4m3_f16(w0, 0), a1 = e4m3_f16(w0, 1), a2 = e4m3_f16(w1, 0), a3 = e4m3_f16(w1, 1);
+          uint32_t a0, a1, a2, a3;
+          e4m3x4_f16(u ? h0 : l0, a0, a1);
+          e4m3x4_f16(u ? h1 : l1, a2, a3);
 #pragma unroll
           for (int n = 0; n < NT; ++n) win_mma<true>(o[n][2 * i + u], a0, a1, a2, a3, b[n][0], b[n][1]);
         }

@@ -2,23 +2,29 @@
 // accumulators): bf16 queries over bf16 / E4M3 / MXFP8 pages, head dims 64
 // and 128.
 //
-// A work item is (sequence, KV head, 256 query rows): the rows of 256 / g new
-// tokens, so the visible pages of an item are those of its first row's window
-// up to its last row's position, plus the pages of the first tokens. Persistent
-// CTAs, one per SM, take the items in a fixed order, long ones (late rows)
-// first, the direction of every second round reversed; nothing is planned on
-// the host. The rows form two 128-row sub-tiles A and B that share each K/V
-// tile of 128 tokens (8 pages of the item's list):
-//   warp 0       TMA producer, two boxes a page into the K/V ring (FP8 codes:
-//                into a staging ring); lane p < 8 looks page p of a tile up
-//   warp 1       issues the products, per tile P_A.V, Q_A.K', P_B.V, Q_B.K'
-//                (the tensor core works on one sub-tile while the softmax of
-//                the other runs)
-//   warps 2-9    softmax, a thread per row: scores from TMEM, one pass per 64
-//                tokens, weights written over them
-//   warps 10-13  FP8: codes widened into the K/V ring
-// The tensor pipe and the exponential unit bound it together: 256 rows x 128
-// tokens are 2048 cycles of products at D = 128 and 2048 of exponentials.
+// A work item is (sequence, KV head, two sub-tiles of 128 / g new tokens), a
+// sub-tile's rows being (token, query head of the group): up to 128 rows of Q,
+// which one TMA box brings. The item's pages are those that its first token's
+// window up to its last token's position reach, plus those of the first tokens.
+// Persistent CTAs, one per SM, take the items in a fixed order, long ones (late
+// tokens) first, the direction of every second round reversed; nothing is
+// planned on the host. K and V come in tiles of 128 tokens (8 pages of the
+// item's list):
+//   softmax      warps 0-3 sub-tile A, 4-7 B, a thread per row: the maximum of
+//                128 scores in TMEM, then the weights of the tile's second and
+//                first 64 tokens, each written over its scores and handed over
+//                by itself
+//   converters   warps 8-11 (FP8): codes widened into the K/V ring
+//   producer     TMA boxes of K and V into the ring (FP8 codes: into a staging
+//                ring); lane p < 8 looks page p of a tile up
+//   issuers      one per sub-tile: per tile P.V by halves, then the next Q.K
+//   scheduler    the items, one ahead, into a small ring that the others read
+//                (finding an item is a chain of dependent loads and divisions),
+//                and an item's Q once the previous item's last scores are done
+// The tensor core works on one sub-tile while the softmax of the other runs.
+// A tile of 256 rows is 2080 cycles of products at D = 128 (65 each, their
+// shared-memory operands keeping that memory busy throughout) and 2048 of
+// exponentials.
 //
 // Types. bf16 and MXFP8 pages take bf16 products; a code times its power of
 // two is exact in bf16. E4M3 pages take f16 products on the bare codes (exact,
@@ -31,9 +37,9 @@
 //
 // Masks. The item's page list is a virtual axis x (first-token pages, then
 // window pages); a row of position p sees x in [p - window + 1 - shift, p -
-// shift] and x < sinks. Only tiles that some row does not see whole are masked;
-// V of slots that no row of the item sees is zeroed before the product (zero
-// times NaN is not zero).
+// shift] and x < sinks. Only chunks that some row does not see whole are
+// masked; V of slots that no row of the item sees is zeroed before the product
+// (zero times NaN is not zero).
 #include <algorithm>
 
 #include "tc_common.cuh"
@@ -41,9 +47,9 @@
 
 namespace dd {
 
-constexpr int kWtRows = 256;
 constexpr int kWtConvWarps = 4;
 constexpr int kWtStages = 3;
+constexpr int kWtChunk = 64;  // tokens of a half tile
 
 template <int D, int KV>
 struct WtCfg {
@@ -55,9 +61,9 @@ struct WtCfg {
   static constexpr int kSlots = kFp8 ? 3 : 4;
   static constexpr int kCodes = kTcTok * D;              // staged codes of a tile
   static constexpr int kExps = kTcTok * (D / 32);        // MXFP8 exponents of a tile
-  static constexpr int kThreads = kFp8 ? 320 + 32 * kWtConvWarps : 320;
-  static constexpr int kSmem = (2 + kSlots) * kTileBytes +
-                               (kFp8 ? kWtStages * (kCodes + kExps) : 0) + 1024;
+  static constexpr int kProducer = kFp8 ? 12 : 8;        // then two issuers and the scheduler
+  static constexpr int kThreads = 32 * (kProducer + 4);
+  static constexpr int kSmem = (2 + kSlots) * kTileBytes + (kFp8 ? kWtStages * (kCodes + kExps) : 0) + 1024;
   // D f32, M = 128; A / B type in bits 7 and 10 (0 f16, 1 bf16); N in bits 17-22.
   static constexpr uint32_t kType = kF16 ? 0u : (1u << 7) | (1u << 10);
   static constexpr uint32_t kIdQK = (1u << 4) | kType | ((128u >> 3) << 17) | ((128u >> 4) << 24);
@@ -68,62 +74,64 @@ struct WtCfg {
   static constexpr float kShift = kF16 ? 7.f : 0.f;
 };
 
+struct WtItem {
+  int32_t ntok;           // new tokens; 0: no such item, -1 in the ring: no more
+  int32_t h;
+  int32_t t0, table;      // the sequence's page table
+  int32_t row;            // first row of q and out
+  int32_t p_lo, p_hi;     // positions of its first and last token
+  WinPages wp;
+  int32_t shift, nchunks;
+};
+
+constexpr int kWtItems = 2;  // items of the ring
 struct WtBars {
   uint64_t kv_full[4], kv_empty[4];
   uint64_t st_full[kWtStages], st_empty[kWtStages];
-  uint64_t s_full[2], p_full[2];
-  uint64_t item_done, q_ready;
+  uint64_t s_full[2];                   // per sub-tile: scores ready (and the previous P.V in O)
+  uint64_t p_full[2][2];                // and half of the tile: weights ready
+  uint64_t o_full[2];                   // once an item: its last P.V is in O
+  uint64_t turn[2];                     // the other sub-tile's products of a tile are issued
+  uint64_t q_raw[2];                    // f16: bf16 rows of Q in place, to be converted
+  uint64_t q_full[2], q_empty[2];       // Q ready / the item's last scores done
+  uint64_t item_full[kWtItems], item_empty[kWtItems];
+  WtItem items[kWtItems];
   uint32_t tmem_base;
   int abort;
 };
 
-struct WtItem {
-  int32_t h, nrows;       // nrows <= 0: no such item
-  int32_t t0, table;      // the sequence's page table
-  int32_t r0;             // first row of the sequence
-  int64_t row0;           // first of the item's rows, counted from the sequence's first
-  int32_t pos0;           // position of the sequence's first row
-  int32_t p_lo, p_hi;
-  WinPages wp;
-  int32_t shift, ntiles;
-};
-
-// Item `i` of this CTA (all roles walk the same list); false past the end.
-__device__ __forceinline__ bool wt_item(const WinArgs& a, int64_t units, int i, WtItem& it) {
-  const int64_t n = gridDim.x;
-  const int64_t u = i * n + ((i & 1) ? n - 1 - blockIdx.x : blockIdx.x);
-  if (i * n >= units) return false;
-  it.nrows = 0;
+// Item `i` of this CTA; false past the end. Tiles are counted in tokens: `per`
+// of them make an item. The launch keeps units and rows * g below 2^31.
+__device__ __forceinline__ bool wt_item(const WinArgs& a, int32_t units, int32_t per, int32_t i, WtItem& it) {
+  const int32_t n = (int32_t)gridDim.x, first = i * n;
+  if (first >= units) return false;
+  const int32_t u = first + ((i & 1) ? n - 1 - (int32_t)blockIdx.x : (int32_t)blockIdx.x);
+  it.ntok = 0;
   if (u >= units) return true;
-  const int64_t unit = units - 1 - u;
-  it.h = (int32_t)(unit % a.Hkv);
+  const uint32_t unit = (uint32_t)(units - 1 - u), tile_id = unit / (uint32_t)a.Hkv;
+  it.h = (int32_t)(unit - tile_id * (uint32_t)a.Hkv);
   int32_t s, tile;
-  win_tile(a, kWtRows, unit / a.Hkv, s, tile);
+  win_tile(a, 1, per, tile_id, s, tile);
   const SeqRows sr = seq_rows(a.row_indptr, a.num_tokens, a.num_rows, s);
-  it.row0 = (int64_t)tile * kWtRows;
-  it.nrows = (int32_t)min((int64_t)kWtRows, max((int64_t)sr.m * a.g - it.row0, (int64_t)0));
-  if (tile < 0) it.nrows = 0;
-  if (it.nrows <= 0) return true;
-  it.r0 = sr.r0;
-  it.pos0 = sr.pos0;
-  it.p_lo = sr.pos0 + (int32_t)(it.row0 / a.g);
-  it.p_hi = sr.pos0 + (int32_t)((it.row0 + it.nrows - 1) / a.g);
+  if (tile < 0 || tile > sr.m / per) return true;
+  it.ntok = min(per, sr.m - tile * per);
+  if (it.ntok <= 0) return true;
+  it.row = sr.r0 + tile * per;
+  it.p_lo = sr.pos0 + tile * per;
+  it.p_hi = it.p_lo + it.ntok - 1;
   it.t0 = a.page_indptr[s];
   it.table = a.page_indptr[s + 1] - it.t0;
   it.wp = win_pages(a.window, a.sinks, it.p_lo, it.p_hi);
   it.shift = (it.wp.wp - it.wp.ns) * kPageSize;
-  it.ntiles = (it.wp.count + kTcPagesPerTile - 1) / kTcPagesPerTile;
+  it.nchunks = (it.wp.count + kWtChunk / kPageSize - 1) / (kWtChunk / kPageSize);
   return true;
 }
-// Pool page of page v of the item's list; 0xFFFFFFFF past its end or where
-// there is no such page.
-__device__ __forceinline__ uint32_t wt_page(const WinArgs& a, const WtItem& it, int32_t v, bool report) {
-  if (v >= it.wp.count) return 0xFFFFFFFFu;
+// Table entry of page v of the item's list as it stands (0xFFFFFFFF past the
+// list or the table): looked up a tile ahead, and judged when it is used, so
+// that nobody waits for it.
+__device__ __forceinline__ uint32_t wt_entry(const WinArgs& a, const WtItem& it, int32_t v) {
   const int32_t idx = it.wp.page(v);
-  const uint32_t id = idx < it.table ? (uint32_t)a.page_indices[it.t0 + idx] : 0xFFFFFFFFu;
-  if (id < (uint32_t)a.num_pages) return id;
-  if (report) win_report(a.status, kDevErrBadPage, idx < it.table ? id : (uint32_t)idx);
-  return 0xFFFFFFFFu;
+  return v < it.wp.count && idx < it.table ? (uint32_t)a.page_indices[it.t0 + idx] : 0xFFFFFFFFu;
 }
 // Whether some row of the item sees virtual token x.
 __device__ __forceinline__ bool wt_seen(const WinArgs& a, const WtItem& it, int32_t x) {
@@ -135,50 +143,132 @@ __device__ __forceinline__ bool wt_whole(const WinArgs& a, const WtItem& it, int
          (a.window == 0 || x > it.p_hi - a.window - it.shift || x + n <= a.sinks);
 }
 
-// Weights of 64 scores, to the products' type, over the chunk's half of the
-// score columns; their f32 sum is added to acc.
-template <bool kF16>
-__device__ __forceinline__ void wt_weights(float (&s)[64], uint64_t sc2, uint64_t nm2, uint64_t& acc, uint32_t taddr) {
-  uint64_t a0 = 0ull, a1 = 0ull;
-#pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const int k = 32 * half + i;
-      const uint64_t x0 = f2_fma(f2_pack(s[k], s[k + 1]), sc2, nm2);
-      const uint64_t x1 = f2_fma(f2_pack(s[k + 2], s[k + 3]), sc2, nm2);
-      const float e0 = fast_exp2(f2_lo(x0)), e1 = fast_exp2(f2_hi(x0));
-      const float e2 = fast_exp2(f2_lo(x1)), e3 = fast_exp2(f2_hi(x1));
-      a0 = f2_add(a0, f2_pack(e0, e1));
-      a1 = f2_add(a1, f2_pack(e2, e3));
-      w[i / 2] = kF16 ? pack_f16x2(e0, e1) : pack_bf16x2(e0, e1);
-      w[i / 2 + 1] = kF16 ? pack_f16x2(e2, e3) : pack_bf16x2(e2, e3);
-    }
-    tmem_st16u(taddr + 16 * half, w);
-  }
-  acc = f2_add(acc, f2_add(a0, a1));
+// One arrival for a warp that is through with something (32 would queue up at
+// the barrier's address).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
-// `cols` columns of packed f16 pairs of this thread's TMEM lane, times f.
-__device__ __noinline__ void tmem_scale_f16(uint32_t taddr, int cols, float f) {
-  for (int c = 0; c < cols; c += 16) {
+// The same value in every lane, known as such.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+
+// Whole-warp forms: one elected lane (the same for every call) issues.
+__device__ __forceinline__ void umma_commit_one(uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred l;\n elect.sync _|l, 0xffffffff;\n"
+      " @l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar))
+      : "memory");
+}
+// Shared-memory descriptors: 128-byte swizzle, 1024 bytes from 8 rows to the
+// next 8; the leading offset and the start address, in 16-byte units, make the
+// low word.
+constexpr uint32_t kWtDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+// S = Q K^T: D / 16 products, 16 dims (32 bytes) apart, 64-dim halves `half` apart.
+template <int D, uint32_t kId>
+__device__ __forceinline__ void umma_qk(uint32_t d, uint32_t a, uint32_t b, uint32_t half) {
+  a |= 1u << 16;
+  b |= 1u << 16;
+#pragma unroll
+  for (int h = 0; h < D / 64; ++h)
+    asm volatile(
+        "{\n .reg .pred l, t, f;\n .reg .b64 da, db;\n .reg .b32 a, b;\n"
+        " elect.sync _|l, 0xffffffff;\n setp.ne.b32 f, %5, 0;\n setp.eq.b32 t, 0, 0;\n"
+        " mov.b64 da, {%1, %3};\n mov.b64 db, {%2, %3};\n"
+        " @l tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, f;\n"
+        " add.u32 a, %1, 2;\n add.u32 b, %2, 2;\n mov.b64 da, {a, %3};\n mov.b64 db, {b, %3};\n"
+        " @l tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, t;\n"
+        " add.u32 a, %1, 4;\n add.u32 b, %2, 4;\n mov.b64 da, {a, %3};\n mov.b64 db, {b, %3};\n"
+        " @l tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, t;\n"
+        " add.u32 a, %1, 6;\n add.u32 b, %2, 6;\n mov.b64 da, {a, %3};\n mov.b64 db, {b, %3};\n"
+        " @l tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, t;\n}" ::"r"(d),
+        "r"(a + h * half), "r"(b + h * half), "n"(kWtDescHi), "n"(kId), "r"(h));
+}
+// O += P V over 64 tokens: 4 products, P 8 TMEM columns and V 16 rows (2 KB) apart.
+template <uint32_t kId>
+__device__ __forceinline__ void umma_pv(uint32_t d, uint32_t p, uint32_t b, uint32_t half, uint32_t acc) {
+  b |= half << 16;
+  asm volatile(
+      "{\n .reg .pred l, t, f;\n .reg .b64 db;\n .reg .b32 b, p;\n"
+      " elect.sync _|l, 0xffffffff;\n setp.ne.b32 f, %5, 0;\n setp.eq.b32 t, 0, 0;\n"
+      " mov.b64 db, {%2, %3};\n"
+      " @l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, f;\n"
+      " add.u32 p, %1, 8;\n add.u32 b, %2, 128;\n mov.b64 db, {b, %3};\n"
+      " @l tcgen05.mma.cta_group::1.kind::f16 [%0], [p], db, %4, t;\n"
+      " add.u32 p, %1, 16;\n add.u32 b, %2, 256;\n mov.b64 db, {b, %3};\n"
+      " @l tcgen05.mma.cta_group::1.kind::f16 [%0], [p], db, %4, t;\n"
+      " add.u32 p, %1, 24;\n add.u32 b, %2, 384;\n mov.b64 db, {b, %3};\n"
+      " @l tcgen05.mma.cta_group::1.kind::f16 [%0], [p], db, %4, t;\n}" ::"r"(d),
+      "r"(p), "r"(b), "n"(kWtDescHi), "n"(kId), "r"(acc));
+}
+// 4-D TMA load (Q rows: dims, heads, head groups, tokens).
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z,
+                                            int32_t w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void prefetch_tma_4d(const CUtensorMap* map, int32_t x, int32_t y, int32_t z, int32_t w) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(x), "r"(y),
+               "r"(z), "r"(w)
+               : "memory");
+}
+
+// 64 bytes of this thread's row of out: whole 32-byte sectors at a time where
+// the address allows (16 bytes at a time are twice the requests, and the rows
+// of a warp are as many lines apart: 6700 against 4400 cycles an item).
+__device__ __forceinline__ void store16(uint16_t* out, const uint32_t (&w)[16], bool wide) {
+  if (wide) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + 16 * k), "r"(w[8 * k]),
+                   "r"(w[8 * k + 1]), "r"(w[8 * k + 2]), "r"(w[8 * k + 3]), "r"(w[8 * k + 4]), "r"(w[8 * k + 5]),
+                   "r"(w[8 * k + 6]), "r"(w[8 * k + 7])
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      reinterpret_cast<uint4*>(out)[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+  }
+}
+
+// This thread's O row times f (rare: kept small rather than fast).
+template <int D>
+__device__ __forceinline__ void wt_rescale(uint32_t taddr, float f) {
+#pragma unroll 1
+  for (int c = 0; c < D; c += 16) {
     uint32_t v[16];
     tmem_ld16u(taddr + c, v);
     tmem_wait_ld();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
-      v[i] = pack_f16x2(x.x * f, x.y * f);
-    }
+    for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
     tmem_st16u(taddr + c, v);
   }
   tmem_wait_st();
 }
 
+// Weights of 32 scores, to the products' type; their f32 sum is added to acc.
+template <bool kF16>
+__device__ __forceinline__ void wt_weights(const float (&s)[32], uint64_t sc2, uint64_t nm2, uint64_t& acc, uint32_t taddr) {
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint64_t x = f2_fma(f2_pack(s[2 * i], s[2 * i + 1]), sc2, nm2);
+    const uint64_t e = f2_pack(fast_exp2(f2_lo(x)), fast_exp2(f2_hi(x)));
+    acc = f2_add(acc, e);
+    w[i] = kF16 ? pack_f16x2(f2_lo(e), f2_hi(e)) : pack_bf16x2(f2_lo(e), f2_hi(e));
+  }
+  tmem_st16u(taddr, w);
+}
+
 template <int D, int KV>
 __global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
-    win_tc_kernel(const __grid_constant__ CUtensorMap kv_map, WinArgs a, int64_t units) {
+    win_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, WinArgs a,
+                  int32_t units) {
   using Cfg = WtCfg<D, KV>;
   constexpr bool kFp8 = Cfg::kFp8, kF16 = Cfg::kF16;
   constexpr int kSlots = Cfg::kSlots, kTile = Cfg::kTileBytes, kHalf = Cfg::kHalfBytes;
@@ -190,57 +280,338 @@ __global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
   uint8_t* stages = slots + kSlots * kTile;   // FP8: [stage][128 rows][D]
   uint8_t* stage_exps = stages + kWtStages * Cfg::kCodes;  // [stage][128 rows][D / 32]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = 128 / a.g;  // tokens of a sub-tile
   WsHeader* err = reinterpret_cast<WsHeader*>(a.status);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) {
-      mbar_init(&bars.kv_full[s], kFp8 ? 32 * kWtConvWarps : 1);
-      mbar_init(&bars.kv_empty[s], 1);
+      mbar_init(&bars.kv_full[s], kFp8 ? kWtConvWarps : 1);
+      mbar_init(&bars.kv_empty[s], 2);  // both sub-tiles' issuers
     }
     for (int s = 0; s < kWtStages; ++s) {
       mbar_init(&bars.st_full[s], 1);
-      mbar_init(&bars.st_empty[s], 32 * kWtConvWarps);
+      mbar_init(&bars.st_empty[s], kWtConvWarps);
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&bars.s_full[x], 1);
-      mbar_init(&bars.p_full[x], 128);
+      for (int h = 0; h < 2; ++h) mbar_init(&bars.p_full[x][h], 4);
+      mbar_init(&bars.o_full[x], 1);
+      mbar_init(&bars.turn[x], 1);
+      mbar_init(&bars.q_raw[x], 1);
+      mbar_init(&bars.q_full[x], kF16 ? 4 : 1);
+      mbar_init(&bars.q_empty[x], 1);
     }
-    mbar_init(&bars.item_done, 1);
-    mbar_init(&bars.q_ready, 256);
+    for (int s = 0; s < kWtItems; ++s) {
+      mbar_init(&bars.item_full[s], 1);
+      mbar_init(&bars.item_empty[s], 8 + (kFp8 ? kWtConvWarps : 0) + 3);
+    }
     bars.abort = 0;
     fence_mbar_init();
+    mbar_arrive(&bars.turn[0]);  // sub-tile A begins
   }
-  if (warp == 1) {
+  if (warp == Cfg::kProducer + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&bars.tmem_base)),
                  "r"(kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (threadIdx.x == 64) prefetch_tmap(&kv_map);
+  if (threadIdx.x == Cfg::kProducer * 32) {
+    prefetch_tmap(&kv_map);
+    prefetch_tmap(&q_map);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = bars.tmem_base;
   volatile int* abort = &bars.abort;
+  // A warp's view of the item ring: the next item, or ntok = -1 after the last
+  // one (and after an abort). The slot is given back once the warp has copied it.
+  int item_k = 0;
+  auto next_item = [&](WtItem& it) {
+    const int s = item_k % kWtItems;
+    const bool got = __all_sync(0xffffffffu, mbar_wait(&bars.item_full[s], (item_k / kWtItems) & 1, abort, err));
+    it = bars.items[s];
+    if (!got) it.ntok = -1;
+    __syncwarp();
+    if (got && lane == 0) mbar_arrive(&bars.item_empty[s]);
+    ++item_k;
+    return it.ntok > 0;
+  };
   WtItem it;
 
-  if (warp == 0) {
+  if (warp < 8) {
+    // ----------------------------------------------------------------- softmax
+    const int x = warp >> 2;        // sub-tile
+    const int quarter = warp & 3;   // TMEM lanes [32 * quarter, + 32)
+    const int r = quarter * 32 + lane;
+    const int tok = x * sub + r / a.g, head = r % a.g;  // this thread's token of an item, head of the group
+    const uint32_t lane_base = tbase + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_col = lane_base + col_s(x), o_col = lane_base + col_o(x);
+    float scale_log2 = a.scale_log2, v_scale = 1.f;  // of the current item
+    int g0 = 0;                // ring index of the item's first K tile
+    int n = 0;                 // items of this sub-tile so far
+    int tiles = 0;             // its tiles so far
+    bool ok = true;
+    // f16: this thread's row of the item's Q, bf16 as loaded, to f16 in place;
+    // returns the power of two that it was multiplied by.
+    auto convert_q = [&]() {
+      int up = 0;
+      if constexpr (kF16) {
+        ok = mbar_wait(&bars.q_raw[x], n & 1, abort, err) && ok;
+        uint8_t* qx = q_s + x * kTile + r * 128;
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 v = *reinterpret_cast<const uint4*>(qx + (c >> 3) * kHalf + (((c & 7) ^ (r & 7)) << 4));
+          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
+        }
+        up = f16_row_shift(top);
+        const float by = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          uint4* at = reinterpret_cast<uint4*>(qx + (c >> 3) * kHalf + (((c & 7) ^ (r & 7)) << 4));
+          uint4 v = *at;
+          v.x = bf16x2_to_f16x2(v.x, by);
+          v.y = bf16x2_to_f16x2(v.y, by);
+          v.z = bf16x2_to_f16x2(v.z, by);
+          v.w = bf16x2_to_f16x2(v.w, by);
+          *at = v;
+        }
+        fence_proxy_async_smem();
+        warp_arrive(&bars.q_full[x]);
+      }
+      return up;
+    };
+    auto is_active = [&](const WtItem& q) { return q.nchunks > 0 && q.ntok > x * sub; };
+    bool have = next_item(it);
+    int up = have && is_active(it) ? convert_q() : 0;
+    while (have) {
+      const WtItem cur = it;
+      const bool active = is_active(cur);
+      if constexpr (kF16) {
+        scale_log2 = f16_score_scale(a.scale_log2, up) * reinterpret_cast<const float*>(a.scales)[cur.h];
+        v_scale = reinterpret_cast<const float*>(a.scales)[a.Hkv + cur.h];
+      }
+      const int32_t p = cur.p_lo + tok;
+      const int32_t hi = p - cur.shift, lo = a.window ? p - a.window + 1 - cur.shift : 0;
+      const int nchunks = active ? cur.nchunks : 0;
+      const int pj = lane & (kTcPagesPerTile - 1);
+      uint32_t entry = nchunks > 0 ? wt_entry(a, cur, pj) : 0xFFFFFFFFu;
+      float m_used = -INFINITY;
+      uint64_t lsum = 0ull;
+      const uint64_t sc2 = f2_pack(scale_log2, scale_log2);
+      for (int c = 0; c < nchunks; c += 2) {
+        const int32_t x0 = c * kWtChunk;
+        const bool two = c + 1 < nchunks;
+        // Which of the tile's pages exist.
+        const uint32_t pages = __ballot_sync(0xffffffffu, entry < (uint32_t)a.num_pages) & 0xffu;
+        entry = wt_entry(a, cur, (c / 2 + 1) * kTcPagesPerTile + pj);
+        const bool seen_whole = wt_whole(a, cur, x0, kTcTok), whole = pages == 0xffu && seen_whole;
+        float s[2][32];
+        // Scores of half h, those that the row does not see as -inf.
+        auto load = [&](int h) {
+          tmem_ld32(s_col + kWtChunk * h, s[0]);
+          tmem_ld32(s_col + kWtChunk * h + 32, s[1]);
+          tmem_wait_ld();
+          if (whole) return;
+          auto below = [](int32_t n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {  // bit k: the row sees token x0 + 64 h + 32 i + k
+            const int32_t b = x0 + kWtChunk * h + 32 * i;
+            uint32_t see = below(hi - b + 1) & (~below(lo - b) | below(a.sinks - b));
+            if (!((pages >> (4 * h + 2 * i)) & 1)) see &= 0xffff0000u;
+            if (!((pages >> (4 * h + 2 * i + 1)) & 1)) see &= 0x0000ffffu;
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (!((see >> k) & 1)) s[i][k] = -INFINITY;
+          }
+        };
+        // (A NaN or infinite score passes the maximum by or makes it infinite;
+        // its exponential is NaN either way, and with it the row's sum.)
+        auto row_max = [&]() {
+          float mx[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float* v = &s[i / 2][16 * (i % 2)];
+            mx[i] = fmaxf(v[0], v[1]);
+#pragma unroll
+            for (int k = 2; k < 16; k += 2) mx[i] = max3f(mx[i], v[k], v[k + 1]);
+          }
+          return max3f(fmaxf(mx[0], mx[1]), mx[2], mx[3]);
+        };
+        ok = ok && mbar_wait(&bars.s_full[x], tiles & 1, abort, err);
+        ++tiles;
+        tc_fence_after();
+        load(0);
+        float mt = row_max();
+        if (two) {
+          load(1);
+          mt = fmaxf(mt, row_max());
+        }
+        mt = ok ? mt * scale_log2 : m_used;
+        if (__any_sync(0xffffffffu, mt > m_used + Cfg::kStep)) {
+          const float m_new = mt > m_used + Cfg::kStep ? ceilf(mt) : m_used;
+          const float f = m_used == m_new ? 1.f : exp2f(m_used - m_new);  // a power of two
+          if (c > 0) wt_rescale<D>(o_col, f);
+          lsum = f2_fma(lsum, f2_pack(f, f), 0ull);
+          m_used = m_new;
+        }
+        // bf16 pages: V of slots that no row sees, before any of the tile's
+        // products (each sub-tile's threads for itself, a token each).
+        if (!kFp8 && !seen_whole) {
+          const int vi = g0 + c + 1;
+          ok = mbar_wait(&bars.kv_full[vi % kSlots], (vi / kSlots) & 1, abort, err) && ok;
+          if (!wt_seen(a, cur, x0 + r)) {
+            uint8_t* v = slots + (vi % kSlots) * kTile + r * 128;
+#pragma unroll
+            for (int hf = 0; hf < Cfg::kHalves; ++hf)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(v + hf * kHalf + 16 * k) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        const float ref = (m_used == -INFINITY ? 0.f : m_used) - Cfg::kShift;
+        const uint64_t nm2 = f2_pack(-ref, -ref);
+        auto hand_over = [&](int h) {
+          wt_weights<kF16>(s[0], sc2, nm2, lsum, s_col + kWtChunk * h);
+          wt_weights<kF16>(s[1], sc2, nm2, lsum, s_col + kWtChunk * h + 16);
+          tmem_wait_st();
+          tc_fence_before();
+          warp_arrive(&bars.p_full[x][h]);
+        };
+        if (two) {
+          hand_over(1);
+          load(0);  // again: 64 registers hold a half at a time
+        }
+        hand_over(0);
+      }
+      g0 += 2 * ((cur.nchunks + 1) / 2);
+      if (active) ++n;
+      have = next_item(it);
+      // The next item's Q before this epilogue: its first scores overlap it
+      // (its first P.V, which overwrites O, waits for this thread's weights).
+      const int up_next = have && is_active(it) ? convert_q() : 0;
+      if (active) {
+        ok = mbar_wait(&bars.o_full[x], (n - 1) & 1, abort, err) && ok;
+        __syncwarp();
+        tc_fence_after();
+      }
+      {
+        const bool live = r < sub * a.g && tok < cur.ntok, wide = ((uintptr_t)a.out & 31) == 0;
+        const float L = f2_lo(lsum) + f2_hi(lsum);
+        const float inv = L == 0.f ? 0.f : v_scale / L;
+        const int64_t dst = (int64_t)(cur.row + tok) * a.Hq + qo_head_of(a.gqa_map, cur.h, head, a.Hkv, a.g);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          if (active) {
+            tmem_ld32(o_col + c * 32, o);
+            tmem_wait_ld();
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = 0.f;
+          }
+          if (live) {
+            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + dst * D + c * 32;
+            uint32_t w[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) w[k] = pack_bf16x2(o[2 * k] * inv, o[2 * k + 1] * inv);
+            store16(out, w, wide);
+          }
+        }
+        if (live && a.lse)
+          a.lse[dst] = L == 0.f ? -INFINITY : (m_used - Cfg::kShift + log2f(L)) * kLn2;
+      }
+      up = up_next;
+      tc_fence_before();
+      if (!__all_sync(0xffffffffu, ok)) break;
+    }
+  } else if (kFp8 && warp < 12) {
+    // -------------------------------------------------------------- converters
+    // A thread widens 16 codes of one token at a time; eight neighbouring
+    // threads cover two rows, so their stores fall into eight bank groups.
+    const int t = threadIdx.x - 256;
+    constexpr int kConvThreads = 32 * kWtConvWarps;
+    constexpr int kChunks = kTcTok * D / 16;
+    int gidx = 0;
+    bool ok = true;
+    while (ok && next_item(it)) {
+      const int pj = lane & (kTcPagesPerTile - 1);
+      uint32_t entry = wt_entry(a, it, pj), pages = 0;
+      const int ntiles = (it.nchunks + 1) / 2;
+      for (int idx = 0; idx < 2 * ntiles; ++idx, ++gidx) {
+        const int su = gidx % kWtStages, s = gidx % kSlots;
+        if ((idx & 1) == 0) {  // the tile's pages that exist; the next tile's ids on their way
+          pages = __ballot_sync(0xffffffffu, entry < (uint32_t)a.num_pages);
+          entry = wt_entry(a, it, ((idx >> 1) + 1) * kTcPagesPerTile + pj);
+        }
+        ok = mbar_wait(&bars.st_full[su], (gidx / kWtStages) & 1, abort, err) &&
+             (gidx < kSlots || mbar_wait(&bars.kv_empty[s], ((gidx / kSlots) - 1) & 1, abort, err));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint8_t* src = stages + su * Cfg::kCodes;
+        const uint8_t* exps = stage_exps + su * Cfg::kExps;
+        uint8_t* dst = slots + s * kTile;
+        const int32_t x0 = (idx >> 1) * kTcTok;
+        const bool clean = (pages & 0xffu) == 0xffu && wt_whole(a, it, x0, kTcTok);
+#pragma unroll 4
+        for (int id = t; id < kChunks; id += kConvThreads) {
+          int row, c;  // token, 16-dim chunk
+          uint4 codes;
+          if constexpr (D == 128) {
+            const int half = (id >> 3) & 1;
+            row = ((id >> 4) << 1) | ((id >> 2) & 1);
+            c = half * 4 + (id & 3);
+            codes = *reinterpret_cast<const uint4*>(src + row * 128 + ((c ^ (row & 7)) << 4));
+          } else {
+            row = id >> 2;
+            c = id & 3;
+            codes = *reinterpret_cast<const uint4*>(src + row * 64 + (c << 4));
+          }
+          uint32_t o[8];
+          if constexpr (kF16) {
+            const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) e4m3x4_f16(w[k], o[2 * k], o[2 * k + 1]);
+          } else {
+            e4m3x16_to_bf16(codes, e8m0_to_float(exps[row * (D / 32) + (c >> 1)]), o);
+          }
+          // Slots that no row sees, and missing pages (their exponents are stale).
+          if (!clean && (!((pages >> (row >> 4)) & 1) || !wt_seen(a, it, x0 + row))) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] = 0;
+          }
+          uint8_t* drow = dst + (c >> 2) * kHalf + row * 128;
+          const int cl = c & 3;
+          *reinterpret_cast<uint4*>(drow + (((2 * cl) ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(drow + (((2 * cl + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+        fence_proxy_async_smem();
+        warp_arrive(&bars.kv_full[s]);
+        if (lane == 0) mbar_arrive(&bars.st_empty[su]);
+      }
+    }
+  } else if (warp == Cfg::kProducer) {
     // ---------------------------------------------------------------- producer
     const int64_t rows_total = (int64_t)a.num_pages * 2 * a.Hkv * kPageSize;
     const int pj = lane & (kTcPagesPerTile - 1);
     const bool mine = lane < kTcPagesPerTile;
     int gidx = 0;
     bool ok = true;
-    for (int i = 0; ok && wt_item(a, units, i, it); ++i) {
-      if (it.nrows <= 0) continue;
-      uint32_t cur = mine ? wt_page(a, it, pj, true) : 0xFFFFFFFFu;
-      uint32_t nxt = 0xFFFFFFFFu;
-      for (int idx = 0; idx < 2 * it.ntiles; ++idx, ++gidx) {
+    while (ok && next_item(it)) {
+      uint32_t cur = wt_entry(a, it, pj), nxt = 0xFFFFFFFFu;
+      const int ntiles = (it.nchunks + 1) / 2;
+      for (int idx = 0; idx < 2 * ntiles; ++idx, ++gidx) {
         const int j = idx >> 1, kv = idx & 1;
-        if (kv == 0 && mine) nxt = wt_page(a, it, (j + 1) * kTcPagesPerTile + pj, true);
         // A missing page reads past the pool's end: zeros.
-        const bool have = mine && cur != 0xFFFFFFFFu;
+        const bool have = mine && cur < (uint32_t)a.num_pages;
+        if (kv == 0 && mine && !have && j * kTcPagesPerTile + pj < it.wp.count) {
+          const int32_t at = it.wp.page(j * kTcPagesPerTile + pj);
+          win_report(a.status, kDevErrBadPage, at < it.table ? cur : (uint32_t)at);
+        }
         const int y = have ? (int)((((int64_t)cur * 2 + kv) * a.Hkv + it.h) * kPageSize) : (int)rows_total;
         if constexpr (kFp8) {
           const int su = gidx % kWtStages;
@@ -272,352 +643,145 @@ __global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
             for (int hf = 0; hf < Cfg::kHalves; ++hf) tma_load_2d(dst + hf * kHalf, &kv_map, 64 * hf, y, &bars.kv_full[s]);
           }
         }
-        if (kv == 1) cur = nxt;
+        if (kv == 0)
+          nxt = wt_entry(a, it, (j + 1) * kTcPagesPerTile + pj);
+        else
+          cur = nxt;
       }
     }
-  } else if (warp == 1) {
-    // -------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
-      const uint64_t q_desc0 = umma_desc(smem_u32(q_s), 16, 1024);
-      const uint64_t k_desc0 = umma_desc(smem_u32(slots), 16, 1024);
-      const uint64_t v_desc0 = umma_desc(smem_u32(slots), kHalf, 1024);
-      int g0 = 0;            // ring index of the item's first K tile
-      int seen[2] = {0, 0};  // tiles each sub-tile's softmax has handed over
-      int n = 0;             // items so far
-      bool ok = true;
-      for (int i = 0; ok && wt_item(a, units, i, it); ++i) {
-        if (it.nrows <= 0) continue;
-        const int ntiles = it.ntiles;
-        const int nsub = it.nrows > 128 ? 2 : 1;
-        auto wait_slot = [&](int idx) {
-          return mbar_wait(&bars.kv_full[(g0 + idx) % kSlots], ((g0 + idx) / kSlots) & 1, abort, err);
-        };
-        auto issue_qk = [&](int x, int j) {
-          const uint64_t kd = k_desc0 + (uint64_t)((((g0 + 2 * j) % kSlots) * kTile) >> 4);
-          const uint64_t qd = q_desc0 + (uint64_t)((x * kTile) >> 4);
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint64_t off = (uint64_t)(((kk >> 2) * kHalf + (kk & 3) * 32) >> 4);
-            umma_ss(tbase + col_s(x), qd + off, kd + off, Cfg::kIdQK, kk > 0 ? 1u : 0u);
-          }
-          umma_commit(&bars.s_full[x]);
-        };
-        ok = mbar_wait(&bars.q_ready, n & 1, abort, err);
-        ++n;
-        if (!ok || ntiles == 0) continue;
-        ok = wait_slot(0);
-        if (!ok) break;
-        tc_fence_after();
-        for (int x = 0; x < nsub; ++x) issue_qk(x, 0);
-        umma_commit(&bars.kv_empty[g0 % kSlots]);
-        for (int j = 0; ok && j < ntiles; ++j) {
-          const int sv = (g0 + 2 * j + 1) % kSlots;
-          const uint64_t vd = v_desc0 + (uint64_t)((sv * kTile) >> 4);
-          for (int x = 0; ok && x < nsub; ++x) {
-            if (!mbar_wait(&bars.p_full[x], (seen[x] + j) & 1, abort, err)) { ok = false; break; }
-            if (x == 0 && !wait_slot(2 * j + 1)) { ok = false; break; }
-            tc_fence_after();
-#pragma unroll
-            for (int kt = 0; kt < 8; ++kt)
-              umma_ts(tbase + col_o(x), tbase + col_s(x) + kt * 8, vd + (uint64_t)((kt * 2048) >> 4), Cfg::kIdPV,
-                      (j > 0 || kt > 0) ? 1u : 0u);
-            if (j + 1 < ntiles) {
-              if (x == 0) {
-                if (!wait_slot(2 * j + 2)) { ok = false; break; }
-                tc_fence_after();
-              }
-              issue_qk(x, j + 1);
-              if (x == nsub - 1) umma_commit(&bars.kv_empty[(g0 + 2 * j + 2) % kSlots]);
-            }
-          }
-          if (ok) umma_commit(&bars.kv_empty[sv]);
-        }
-        if (ok) umma_commit(&bars.item_done);
-        seen[0] += ntiles;
-        if (nsub > 1) seen[1] += ntiles;
-        g0 += 2 * ntiles;
-      }
-    }
-  } else if (kFp8 && warp >= 10) {
-    // -------------------------------------------------------------- converters
-    // A thread widens 16 codes of one token at a time; eight neighbouring
-    // threads cover two rows, so their stores fall into eight bank groups.
-    const int t = threadIdx.x - 320;
-    constexpr int kConvThreads = 32 * kWtConvWarps;
-    constexpr int kChunks = kTcTok * D / 16;
-    int gidx = 0;
+  } else if (warp <= Cfg::kProducer + 2) {
+    // ----------------------------------------------------------------- issuers
+    // A warp for each sub-tile: a product is accepted only when the one before
+    // it has all but run, and even a wait for a barrier that is already complete
+    // costs 85 cycles, so one warp for both left the tensor core idle at every
+    // wait. The whole warp walks the list, every branch taken on a vote, and one
+    // elected lane issues, several products to an asm block.
+    const int x = warp - Cfg::kProducer - 1;
+    const uint32_t q_addr = (smem_u32(q_s) + x * kTile) >> 4, s_addr = smem_u32(slots) >> 4;
+    const uint32_t tb = uniform(tbase);
+    int g0 = 0;              // ring index of the item's first K tile
+    int n = 0;               // items of this sub-tile
+    int turns = 0;           // turns taken
+    int used[2] = {0, 0};    // its first and second halves of tiles
     bool ok = true;
-    for (int i = 0; ok && wt_item(a, units, i, it); ++i) {
-      if (it.nrows <= 0) continue;
-      const int pj = lane & (kTcPagesPerTile - 1);
-      uint32_t page = wt_page(a, it, pj, false), pages = 0;
-      for (int idx = 0; idx < 2 * it.ntiles; ++idx, ++gidx) {
-        const int su = gidx % kWtStages, s = gidx % kSlots;
-        if ((idx & 1) == 0) {  // the tile's pages that exist; the next tile's ids on their way
-          pages = __ballot_sync(0xffffffffu, page != 0xFFFFFFFFu);
-          page = wt_page(a, it, ((idx >> 1) + 1) * kTcPagesPerTile + pj, false);
+    auto wait = [&](uint64_t* bar, int phase) {
+      const bool all = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, abort, err));
+      tc_fence_after();
+      return all;
+    };
+    while (ok) {
+      next_item(it);
+      const int nchunks = uniform(it.nchunks), ntok = uniform(it.ntok);
+      if (ntok <= 0) break;
+      const int ntiles = (nchunks + 1) / 2;
+      if (ntok <= x * sub) {
+        // Nothing to issue here: the tiles are given back as they come.
+        for (int i = g0; ok && i < g0 + 2 * ntiles; ++i) {
+          ok = wait(&bars.kv_full[i % kSlots], i / kSlots);
+          if (ok && lane == 0) mbar_arrive(&bars.kv_empty[i % kSlots]);
+          __syncwarp();
         }
-        ok = mbar_wait(&bars.st_full[su], (gidx / kWtStages) & 1, abort, err) &&
-             (gidx < kSlots || mbar_wait(&bars.kv_empty[s], ((gidx / kSlots) - 1) & 1, abort, err));
-        ok = __all_sync(0xffffffffu, ok);
+        g0 += 2 * ntiles;
+        continue;
+      }
+      if (nchunks == 0) continue;
+      // With both sub-tiles at work their products are issued in turn, a tile's
+      // last P.V and the next Q.K together: issued as they come, both sub-tiles
+      // fall into step, their softmaxes share the exponential unit and then
+      // their products the tensor core (4650 cycles a tile).
+      const bool both = ntok > sub;
+      auto my_turn = [&]() { return !both || wait(&bars.turn[x], turns++); };
+      auto your_turn = [&]() {
+        if (both && lane == 0) mbar_arrive(&bars.turn[1 - x]);
+        __syncwarp();
+      };
+      // Scores of tile j; what is free after them.
+      auto issue_qk = [&](int j) {
+        const int slot = (g0 + 2 * j) % kSlots;
+        umma_qk<D, Cfg::kIdQK>(tb + col_s(x), q_addr, s_addr + (slot * kTile >> 4), kHalf >> 4);
+        umma_commit_one(&bars.s_full[x]);
+        umma_commit_one(&bars.kv_empty[slot]);
+        if (j == ntiles - 1) umma_commit_one(&bars.q_empty[x]);
+      };
+      ok = wait(&bars.q_full[x], n++) && wait(&bars.kv_full[g0 % kSlots], g0 / kSlots) && my_turn();
+      if (!ok) break;
+      issue_qk(0);
+      your_turn();
+      for (int j = 0; ok && j < ntiles; ++j) {
+        const int vi = g0 + 2 * j + 1, ki = vi + 1, slot = vi % kSlots;
+        const uint32_t o = tb + col_o(x), p = tb + col_s(x), v = s_addr + (slot * kTile >> 4);
+        const bool two = 2 * j + 1 < nchunks, more = j + 1 < ntiles;
+        ok = wait(&bars.kv_full[slot], vi / kSlots) && (!more || wait(&bars.kv_full[ki % kSlots], ki / kSlots));
+        if (two) {
+          ok = ok && wait(&bars.p_full[x][1], used[1]++);
+          if (!ok) break;
+          umma_pv<Cfg::kIdPV>(o, p + kWtChunk, v + (kWtChunk * 128 >> 4), kHalf >> 4, j > 0 ? 1u : 0u);
+        }
+        ok = ok && my_turn() && wait(&bars.p_full[x][0], used[0]++);
         if (!ok) break;
-        const uint8_t* src = stages + su * Cfg::kCodes;
-        const uint8_t* exps = stage_exps + su * Cfg::kExps;
-        uint8_t* dst = slots + s * kTile;
-        const int32_t x0 = (idx >> 1) * kTcTok;
-        const bool clean = wt_whole(a, it, x0, kTcTok);
-#pragma unroll 4
-        for (int id = t; id < kChunks; id += kConvThreads) {
-          int row, c;  // token, 16-dim chunk
-          uint4 codes;
-          if constexpr (D == 128) {
-            const int half = (id >> 3) & 1;
-            row = ((id >> 4) << 1) | ((id >> 2) & 1);
-            c = half * 4 + (id & 3);
-            codes = *reinterpret_cast<const uint4*>(src + row * 128 + ((c ^ (row & 7)) << 4));
-          } else {
-            row = id >> 2;
-            c = id & 3;
-            codes = *reinterpret_cast<const uint4*>(src + row * 64 + (c << 4));
-          }
-          uint32_t o[8];
-          if constexpr (kF16) {
-            const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              o[2 * k] = e4m3_f16(w[k], 0);
-              o[2 * k + 1] = e4m3_f16(w[k], 1);
-            }
-          } else {
-            e4m3x16_to_bf16(codes, e8m0_to_float(exps[row * (D / 32) + (c >> 1)]), o);
-          }
-          // Slots that no row sees, and missing pages (their exponents are stale).
-          if (!((pages >> (row >> 4)) & 1) || (!clean && !wt_seen(a, it, x0 + row))) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] = 0;
-          }
-          uint8_t* drow = dst + (c >> 2) * kHalf + row * 128;
-          const int cl = c & 3;
-          *reinterpret_cast<uint4*>(drow + (((2 * cl) ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(drow + (((2 * cl + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(&bars.kv_full[s]);
-        mbar_arrive(&bars.st_empty[su]);
+        umma_pv<Cfg::kIdPV>(o, p, v, kHalf >> 4, j > 0 || two ? 1u : 0u);
+        umma_commit_one(&bars.kv_empty[slot]);
+        if (more)
+          issue_qk(j + 1);
+        else
+          umma_commit_one(&bars.o_full[x]);
+        your_turn();
       }
+      g0 += 2 * ntiles;
     }
-  } else if (warp >= 2 && warp < 10) {
-    // ----------------------------------------------------------------- softmax
-    const int x = (warp - 2) >> 2;  // sub-tile
-    const int quarter = warp & 3;   // TMEM lanes [32 * quarter, + 32)
-    const int r = quarter * 32 + lane, row = x * 128 + r;
-    const uint32_t lane_base = tbase + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_col = lane_base + col_s(x), o_col = lane_base + col_o(x);
-    float scale_log2 = a.scale_log2, v_scale = 1.f;  // of the current item
-    int seen = 0, done = 0, g0 = 0;
-    // Row of q and out that this thread holds of an item.
-    auto place = [&](const WtItem& q, int64_t& token) {
-      const int64_t rr = q.row0 + row;
-      token = q.r0 + rr / a.g;
-      return qo_head_of(a.gqa_map, q.h, (int)(rr % a.g), a.Hkv, a.g);
-    };
-    // Q row -> the sub-tile's swizzled K-major tile, handed to the MMA warp.
-    // Returns the power of two by which the stored row must be multiplied back.
-    auto write_q = [&](const WtItem& q) {
-      const uint4* src = nullptr;
-      if (row < q.nrows) {
-        int64_t token;
-        const int hq = place(q, token);
-        src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + token * a.q_stride + (int64_t)hq * D);
+  } else {
+    // --------------------------------------------------- scheduler and Q loader
+    // Publishes item k + 1 (and asks for its Q in L2), then loads the Q of item
+    // k once the scores of item k - 1 are done.
+    int n[2] = {0, 0};
+    bool ok = true, have = false;
+    const bool tiled = a.gqa_map == DD_GQA_TILED;
+    WtItem nx;
+    it.ntok = 0;
+    for (int i = 0, k = 0;; ++i) {
+      const bool more = wt_item(a, units, 2 * sub, i, nx);
+      if (!more) nx.ntok = -1;
+      if (nx.ntok == 0) continue;
+      const int s = k % kWtItems;
+      ok = __all_sync(0xffffffffu, k < kWtItems || mbar_wait(&bars.item_empty[s], ((k / kWtItems) - 1) & 1, abort, err));
+      if (!ok) break;
+      if (lane == 0) {
+        bars.items[s] = nx;
+        mbar_arrive(&bars.item_full[s]);
+        if (more && nx.nchunks > 0)
+          for (int x = 0; x < 2 && nx.ntok > x * sub; ++x)
+            for (int hf = 0; hf < Cfg::kHalves; ++hf)
+              prefetch_tma_4d(&q_map, 64 * hf, tiled ? nx.h : 0, tiled ? 0 : nx.h, nx.row + x * sub);
       }
-      int up = 0;
-      if constexpr (kF16) {
-        uint32_t top = 0;
+      __syncwarp();
+      ++k;
+      if (have) {
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 v = src ? src[c] : make_uint4(0, 0, 0, 0);
-          const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
-        }
-        up = f16_row_shift(top);
-      }
-      const float by = __uint_as_float((uint32_t)(127 + up) << 23);
-      uint8_t* qx = q_s + x * kTile + r * 128;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 v = src ? src[c] : make_uint4(0, 0, 0, 0);
-        if constexpr (kF16) {
-          v.x = bf16x2_to_f16x2(v.x, by);
-          v.y = bf16x2_to_f16x2(v.y, by);
-          v.z = bf16x2_to_f16x2(v.z, by);
-          v.w = bf16x2_to_f16x2(v.w, by);
-        }
-        *reinterpret_cast<uint4*>(qx + (c >> 3) * kHalf + (((c & 7) ^ (r & 7)) << 4)) = v;
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&bars.q_ready);
-      return up;
-    };
-    int i = 0;
-    bool have = false;
-    while (wt_item(a, units, i, it)) {
-      if (it.nrows > 0) {
-        have = true;
-        break;
-      }
-      ++i;
-    }
-    int up = 0;
-    if (have) up = write_q(it);
-    while (have) {
-      const WtItem cur = it;
-      const bool live = row < cur.nrows, active = x == 0 || cur.nrows > 128;
-      // The next item with rows, if any.
-      have = false;
-      while (wt_item(a, units, ++i, it)) {
-        if (it.nrows > 0) {
-          have = true;
-          break;
-        }
-      }
-      if constexpr (kF16) {
-        scale_log2 = f16_score_scale(a.scale_log2, up) * reinterpret_cast<const float*>(a.scales)[cur.h];
-        v_scale = reinterpret_cast<const float*>(a.scales)[a.Hkv + cur.h];
-      }
-      const int32_t p = cur.pos0 + (int32_t)((cur.row0 + row) / a.g);
-      const int32_t hi = p - cur.shift, lo = a.window ? p - a.window + 1 - cur.shift : 0;
-      const int ntiles = cur.ntiles;
-      // Which of a tile's pages exist: looked up a tile ahead, as the producer does.
-      const int pj = lane & (kTcPagesPerTile - 1);
-      uint32_t page = active && ntiles > 0 ? wt_page(a, cur, pj, false) : 0xFFFFFFFFu;
-      float m_used = -INFINITY;
-      uint64_t lsum = 0ull;
-      bool ok = true;
-      const uint64_t sc2 = f2_pack(scale_log2, scale_log2);
-      for (int j = 0; active && j < ntiles; ++j) {
-        const int32_t x0 = j * kTcTok;
-        const uint32_t pages = __ballot_sync(0xffffffffu, page != 0xFFFFFFFFu) & 0xffu;
-        page = wt_page(a, cur, (j + 1) * kTcPagesPerTile + pj, false);
-        const bool whole = pages == 0xffu && wt_whole(a, cur, x0, kTcTok);
-        ok = ok && mbar_wait(&bars.s_full[x], (seen + j) & 1, abort, err);
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float s[64];
-          {
-            float t[32];
-            tmem_ld32(s_col + c * 64, t);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) s[k] = t[k];
-            tmem_ld32(s_col + c * 64 + 32, t);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) s[32 + k] = t[k];
-          }
-          if (!whole) {
-            // Bit k: the row sees token x0 + 64 c + k.
-            const int32_t b = x0 + 64 * c;
-            auto below = [](int32_t n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
-            uint64_t see = below(hi - b + 1) & (~below(lo - b) | below(a.sinks - b));
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (!((pages >> (4 * c + k)) & 1)) see &= ~(0xffffull << (16 * k));
-            const uint32_t see0 = (uint32_t)see, see1 = (uint32_t)(see >> 32);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              if (!((see0 >> k) & 1)) s[k] = -INFINITY;
-              if (!((see1 >> k) & 1)) s[32 + k] = -INFINITY;
-            }
-          }
-          float m0 = s[0], m1 = s[1];
-#pragma unroll
-          for (int k = 2; k < 62; k += 4) {
-            m0 = max3f(m0, s[k], s[k + 1]);
-            m1 = max3f(m1, s[k + 2], s[k + 3]);
-          }
-          const float mt = ok ? max3f(m0, m1, fmaxf(s[62], s[63])) * scale_log2 : m_used;
-          if (__any_sync(0xffffffffu, mt > m_used + Cfg::kStep)) {
-            const float m_new = mt > m_used + Cfg::kStep ? ceilf(mt) : m_used;
-            const float f = m_used == m_new ? 1.f : exp2f(m_used - m_new);  // a power of two
-            if (j > 0) tmem_scale_cols<false>(o_col, D, f);
-            if (c == 1) {
-              if constexpr (kF16)
-                tmem_scale_f16(s_col, 32, f);
-              else
-                tmem_scale_cols<true>(s_col, 32, f);
-            }
-            lsum = f2_fma(lsum, f2_pack(f, f), 0ull);
-            m_used = m_new;
-          }
-          const float ref = (m_used == -INFINITY ? 0.f : m_used) - Cfg::kShift;
-          wt_weights<kF16>(s, sc2, f2_pack(-ref, -ref), lsum, s_col + c * 32);
-        }
-        // bf16 pages: V of slots that no row sees (sub-tile A's 128 threads, a
-        // token each, before they hand the weights over).
-        if (!kFp8 && x == 0 && !wt_whole(a, cur, x0, kTcTok)) {
-          const int vi = g0 + 2 * j + 1;
-          ok = mbar_wait(&bars.kv_full[vi % kSlots], (vi / kSlots) & 1, abort, err) && ok;
-          if (!wt_seen(a, cur, x0 + r)) {
-            uint8_t* v = slots + (vi % kSlots) * kTile + r * 128;
+        for (int x = 0; x < 2; ++x) {
+          if (it.nchunks == 0 || it.ntok <= x * sub) break;
+          ok = __all_sync(0xffffffffu, n[x] == 0 || mbar_wait(&bars.q_empty[x], (n[x] - 1) & 1, abort, err));
+          if (!ok) break;
+          ++n[x];
+          if (lane == 0) {
+            uint64_t* bar = kF16 ? &bars.q_raw[x] : &bars.q_full[x];
+            mbar_arrive_expect_tx(bar, Cfg::kHalves * sub * a.g * 128);
 #pragma unroll
             for (int hf = 0; hf < Cfg::kHalves; ++hf)
-#pragma unroll
-              for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(v + hf * kHalf + 16 * k) = make_uint4(0, 0, 0, 0);
+              tma_load_4d(q_s + x * kTile + hf * kHalf, &q_map, 64 * hf, tiled ? it.h : 0, tiled ? 0 : it.h,
+                          it.row + x * sub, bar);
           }
-          fence_proxy_async_smem();
+          __syncwarp();
         }
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&bars.p_full[x]);
+        if (!ok) break;
       }
-      if (active) seen += ntiles;
-      g0 += 2 * ntiles;
-      if (ntiles > 0) {
-        ok = mbar_wait(&bars.item_done, done & 1, abort, err) && ok;
-        ++done;
-        tc_fence_after();
-      }
-      // The next item's Q before this epilogue: its first scores overlap it
-      // (its first P.V, which overwrites O, waits for this thread's weights).
-      const int up_next = have && __all_sync(0xffffffffu, ok) ? write_q(it) : 0;
-      if (active) {
-        const float L = f2_lo(lsum) + f2_hi(lsum);
-        const float inv = L == 0.f ? 0.f : v_scale / L;
-        int64_t token = 0;
-        const int hq = live ? place(cur, token) : 0;
-        const int64_t dst = token * a.Hq + hq;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          float o[32];
-          if (ntiles > 0) {
-            tmem_ld32(o_col + c * 32, o);
-            tmem_wait_ld();
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = 0.f;
-          }
-          if (live) {
-            uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + dst * D + c * 32);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              out[k] = make_uint4(pack_bf16x2(o[8 * k] * inv, o[8 * k + 1] * inv),
-                                  pack_bf16x2(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
-                                  pack_bf16x2(o[8 * k + 4] * inv, o[8 * k + 5] * inv),
-                                  pack_bf16x2(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
-          }
-        }
-        if (live && a.lse)
-          a.lse[dst] = L == 0.f ? -INFINITY : (m_used - Cfg::kShift + log2f(L)) * kLn2;
-      }
-      up = up_next;
-      tc_fence_before();
-      if (!__all_sync(0xffffffffu, ok)) break;
+      if (!more) break;
+      it = nx;
+      have = true;
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == Cfg::kProducer + 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(kTmemCols)
                  : "memory");
@@ -626,33 +790,51 @@ __global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
 
 int make_kv_tensor_map(CUtensorMap* map, const void* kv, int64_t num_pages, int Hkv, int D,
                        int elem_bytes, int two_halves);
+int make_q_tensor_map(CUtensorMap* map, const void* q, int64_t rows, int64_t row_stride, int Hq, int Hkv, int D,
+                      int gqa_map, int tokens);
 
 template <int D, int KV>
-static cudaError_t launch_win_tc_t(const CUtensorMap& map, const WinArgs& a, int64_t units, int sms, cudaStream_t st) {
+static cudaError_t launch_win_tc_t(const CUtensorMap& kv, const CUtensorMap& q, const WinArgs& a, int32_t units,
+                                   int sms, cudaStream_t st) {
   using Cfg = WtCfg<D, KV>;
   cudaError_t e = cudaFuncSetAttribute(win_tc_kernel<D, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
   if (e != cudaSuccess) return e;
   ProfScope ps(kProfTc, st);
-  win_tc_kernel<D, KV><<<(unsigned)std::min<int64_t>(units, sms), Cfg::kThreads, Cfg::kSmem, st>>>(map, a, units);
+  win_tc_kernel<D, KV><<<std::min(units, sms), Cfg::kThreads, Cfg::kSmem, st>>>(kv, q, a, units);
   return cudaGetLastError();
 }
 template <int D>
-static cudaError_t launch_win_tc_kv(const CUtensorMap& map, const WinArgs& a, int64_t units, int sms, cudaStream_t st) {
+static cudaError_t launch_win_tc_kv(const CUtensorMap& kv, const CUtensorMap& q, const WinArgs& a, int32_t units,
+                                    int sms, cudaStream_t st) {
   switch (a.kv_dtype) {
-    case DD_DTYPE_BF16: return launch_win_tc_t<D, DD_DTYPE_BF16>(map, a, units, sms, st);
-    case DD_DTYPE_E4M3: return launch_win_tc_t<D, DD_DTYPE_E4M3>(map, a, units, sms, st);
-    default: return launch_win_tc_t<D, DD_DTYPE_MXFP8>(map, a, units, sms, st);
+    case DD_DTYPE_BF16: return launch_win_tc_t<D, DD_DTYPE_BF16>(kv, q, a, units, sms, st);
+    case DD_DTYPE_E4M3: return launch_win_tc_t<D, DD_DTYPE_E4M3>(kv, q, a, units, sms, st);
+    default: return launch_win_tc_t<D, DD_DTYPE_MXFP8>(kv, q, a, units, sms, st);
   }
+}
+
+static int64_t win_tc_units(const WinArgs& a) {
+  return ((int64_t)a.num_seqs + a.num_rows / (2 * (128 / a.g))) * a.Hkv;
+}
+
+// A group has to fit a sub-tile, and the kernel's 32-bit item arithmetic and
+// TMA coordinates have to hold the batch and the pool.
+bool win_tc_fits(const WinArgs& a) {
+  const int64_t pool_rows = (int64_t)a.num_pages * 2 * a.Hkv * kPageSize;
+  return a.D <= 128 && a.g <= 128 && pool_rows > 0 && pool_rows <= 0x7FFFFFFF &&
+         win_tc_units(a) < (1ll << 31) - 1024;
 }
 
 int launch_win_tc(const WinArgs& a, cudaStream_t st) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  CUtensorMap map;
-  const int rc = make_kv_tensor_map(&map, a.kv, a.num_pages, a.Hkv, a.D, a.kv_dtype == DD_DTYPE_BF16 ? 2 : 1, 0);
+  CUtensorMap kv, q;
+  int rc = make_kv_tensor_map(&kv, a.kv, a.num_pages, a.Hkv, a.D, a.kv_dtype == DD_DTYPE_BF16 ? 2 : 1, 0);
+  if (!rc) rc = make_q_tensor_map(&q, a.q, a.num_rows, a.q_stride, a.Hq, a.Hkv, a.D, a.gqa_map, 128 / a.g);
   if (rc) return rc;
-  const int64_t units = (a.num_seqs + (int64_t)a.num_rows * a.g / kWtRows) * a.Hkv;
-  const cudaError_t e = a.D == 64 ? launch_win_tc_kv<64>(map, a, units, sms, st) : launch_win_tc_kv<128>(map, a, units, sms, st);
+  const int32_t units = (int32_t)win_tc_units(a);
+  const cudaError_t e = a.D == 64 ? launch_win_tc_kv<64>(kv, q, a, units, sms, st)
+                                  : launch_win_tc_kv<128>(kv, q, a, units, sms, st);
   if (e != cudaSuccess) return fail(DD_ERR_CUDA, std::string("window attention launch: ") + cudaGetErrorString(e));
   return DD_OK;
 }

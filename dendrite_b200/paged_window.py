@@ -57,7 +57,7 @@ def _check_rows(name: str, t, heads: int, dim: int) -> int:
     if len(shape) != 3 or shape[1] != heads or shape[2] != dim or stride[2] != 1 or \
             (heads > 1 and stride[1] != dim):
         _fail(f"{name} must be [rows][{heads}][{dim}] with dense rows")
-    return stride[0] if shape[0] > 1 else max(stride[0], heads * dim)
+    return stride[0] if shape[0] > 1 else heads * dim
 
 
 def _device(*tensors) -> int:
