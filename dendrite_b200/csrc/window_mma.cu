@@ -153,6 +153,18 @@ __device__ __forceinline__ void load_v(WinFrag<D, KV>& f, const WinArgs& a, uint
     load_exps<D>(e + 8 * (D / 32), f.ev[1]);
   }
 }
+// Byte b of a word of E8M0 exponents as a power of two (0: 0 in place of
+// 2^-127, which no sum of scores sees; 255: infinity).
+__device__ __forceinline__ float exp_byte(uint32_t w, int b) {
+  return __uint_as_float(__byte_perm(w, 0u, 0x0444u | (b << 12)) >> 1);
+}
+template <int N>
+__device__ __forceinline__ bool has_nan_exp(const uint32_t (&e)[N]) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) any |= (~e[i] - 0x01010101u) & e[i] & 0x80808080u;  // a zero byte of ~e
+  return any != 0;
+}
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 __device__ __forceinline__ uint32_t word(const uint2& v, int i) { return i == 0 ? v.x : v.y; }
 
@@ -182,11 +194,12 @@ __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// CTAs an SM holds: FP8 pages are half the bytes of bf16 ones, so it takes more
-// warps to have as many in flight (128 x 2048 tokens of E4M3 / SM at 3 CTAs:
-// 131 us, 4: see the launch rule), as far as the registers go without spills.
+// CTAs that an SM holds, as far as the registers go. FP8 pages are half the
+// bytes of bf16 ones and need the fourth (128 x 2048 tokens of E4M3: 102 us; a
+// second page in flight for each warp of three CTAs 126, five CTAs with spills
+// 140).
 template <int D, int KV, int NT>
-constexpr int kWinCtas = D * NT >= 256 ? 2 : KV != kWinBf16 || D == 64 ? 4 : 3;
+constexpr int kWinCtas = D * NT >= 256 ? 2 : KV == kWinBf16 && D == 128 ? 3 : 4;
 
 template <int D, int KV, int NT>
 __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_kernel(WinArgs a, int nsplit) {
@@ -229,13 +242,22 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
     return 0xFFFFFFFFu;
   };
   uint32_t ids = read_ids(base_v);
-  int32_t at = 0;  // pages done of this read
-  uint32_t page = __shfl_sync(0xffffffffu, ids, 0);
-
+  int32_t at = 0;  // pages handed out of this read
+  // Pages v0 + warp, + kWinWarps, ... one call after another; 0xFFFFFFFF for a bad one.
+  auto take = [&](int32_t v) {
+    if (v >= v1) return 0xFFFFFFFFu;
+    if (at == 32) {
+      base_v = v;
+      ids = read_ids(base_v);
+      at = 0;
+    }
+    return __shfl_sync(0xffffffffu, ids, at++);
+  };
   WinFrag<D, KV> f;
-  if (page != 0xFFFFFFFFu) {
-    load_k<D, KV>(f, a, page, h, g, c);
-    load_v<D, KV>(f, a, page, h, g, c);
+  uint32_t now = take(v0 + warp);
+  if (now != 0xFFFFFFFFu) {
+    load_k<D, KV>(f, a, now, h, g, c);
+    load_v<D, KV>(f, a, now, h, g, c);
   }
 
   // Q fragments: lane (g, c) holds row 8 n + g, dims 32 i + 8 c .. + 8.
@@ -295,21 +317,15 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
 #pragma unroll
   for (int i = 0; i < (D + 127) / 128; ++i) ref_e[i] = 0;
 
+  // Page v of the list, pool page `now`; the loads of the next one go out as
+  // f's registers come free.
   for (int32_t v = v0 + warp; v < v1; v += kWinWarps) {
-    // The next page's id, so its loads can go out as registers free up.
-    uint32_t next;
-    if (++at == 32) {
-      base_v = v + kWinWarps;
-      ids = read_ids(base_v);
-      at = 0;
-    }
-    next = __shfl_sync(0xffffffffu, ids, at);
-    if (v + kWinWarps >= v1) next = 0xFFFFFFFFu;
-    if (page == 0xFFFFFFFFu) {  // a bad page: skipped
-      page = next;
-      if (page != 0xFFFFFFFFu) {
-        load_k<D, KV>(f, a, page, h, g, c);
-        load_v<D, KV>(f, a, page, h, g, c);
+    const uint32_t next = take(v + kWinWarps);
+    if (now == 0xFFFFFFFFu) {  // a bad page: skipped
+      now = next;
+      if (now != 0xFFFFFFFFu) {
+        load_k<D, KV>(f, a, now, h, g, c);
+        load_v<D, KV>(f, a, now, h, g, c);
       }
       continue;
     }
@@ -343,7 +359,7 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
           for (int n = 0; n < NT; ++n) win_mma<true>(y[n], a0, a1, a2, a3, q[n][i][2 * u], q[n][i][2 * u + 1]);
         }
         if constexpr (KV == kWinMx) {
-          const float e0 = e8m0_byte_to_float(f.ek[0][i / 4], i % 4), e1 = e8m0_byte_to_float(f.ek[1][i / 4], i % 4);
+          const float e0 = exp_byte(f.ek[0][i / 4], i % 4), e1 = exp_byte(f.ek[1][i / 4], i % 4);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             x[n][0] = fmaf(y[n][0], e0, x[n][0]);
@@ -359,8 +375,17 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
         }
       }
     }
-    page = next;
-    if (page != 0xFFFFFFFFu) load_k<D, KV>(f, a, page, h, g, c);
+    if constexpr (KV == kWinMx) {
+      // exp_byte takes the NaN exponent for infinity.
+      const bool n0 = has_nan_exp(f.ek[0]), n1 = has_nan_exp(f.ek[1]);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (e < 2 ? n0 : n1) x[n][e] = NAN;
+    }
+    now = next;
+    if (now != 0xFFFFFFFFu) load_k<D, KV>(f, a, now, h, g, c);
     // ---- mask. Most pages are seen whole by every row.
     const int32_t j0 = wp.page(v) * kPageSize;
 #pragma unroll
@@ -506,13 +531,13 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
         if constexpr (KV == kWinMx) {
-          // The block's weights: w * 2^(e - reference); 255 is the NaN exponent.
-          const int top = (int)((ref_e[i / 4] >> (8 * (i % 4))) & 255);
+          // The block's weights: w * 2^(e - reference), 0 where that is below
+          // 2^-126. (A NaN exponent is the reference itself, and makes the block
+          // NaN when it is put back in.)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const int e = (int)((f.ev[half][i / 4] >> (8 * (i % 4))) & 255);
-            const float by = e == 255 ? __uint_as_float(0x7fc00000u)
-                                      : top - e > 126 ? 0.f : __uint_as_float((uint32_t)(127 + e - top) << 23);
+            const uint32_t down = __byte_perm(ref_e[i / 4] - f.ev[half][i / 4], 0u, 0x0444u | ((i % 4) << 12)) >> 1;
+            const float by = __uint_as_float(0x3f800000u - min(down, 127u << 23));
 #pragma unroll
             for (int n = 0; n < NT; ++n)
               b[n][half] = movm_trans(pack_f16x2(x[n][2 * half] * by, x[n][2 * half + 1] * by));
@@ -530,7 +555,7 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
         }
       }
     }
-    if (page != 0xFFFFFFFFu) load_v<D, KV>(f, a, page, h, g, c);
+    if (now != 0xFFFFFFFFu) load_v<D, KV>(f, a, now, h, g, c);
   }
 
   // ---- the warp's state, normalised by its own sum
@@ -629,8 +654,35 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
 }
 
 // ------------------------------------------------------------------ host side
+// CTAs of a cluster. A CTA costs some 6 us of dependent loads and joining
+// besides its pages, so no more than one wave of them is launched, down to a
+// page for each warp; but where the units (tile, KV head) alone are a little
+// more than whole waves and have pages enough, they are split to even the last
+// one out. (4096-token windows, bf16: 64 sequences of 8 heads, 512 units for
+// 444 places: 220 us whole, 187 in two, 177 in four; 4 sequences: 67 us whole,
+// 17 in eight, 28 in sixteen, which is more than one wave.)
+static int win_split(int64_t units, int64_t places, int64_t pages) {
+  int n = 1;
+  while (n < 16 && units * n * 2 <= places && pages >= 2 * n * kWinWarps) n *= 2;
+  auto last_wave_idle = [&]() {
+    const int64_t waves = (units * n + places - 1) / places;
+    return units * n * 100 < waves * places * 85;
+  };
+  if (units > places)
+    while (n < 8 && last_wave_idle() && pages >= 128 * n) n *= 2;
+  return n;
+}
+
 template <int D, int KV, int NT>
-static int launch_win_mma_t(const WinArgs& a, int64_t tiles, int nsplit, cudaStream_t st) {
+static int launch_win_mma_t(const WinArgs& a, int max_pages, int sms, cudaStream_t st) {
+  constexpr int R = 8 * NT;
+  const int64_t tiles = a.row_indptr ? a.num_seqs + (int64_t)a.num_rows * a.g / R
+                                     : (int64_t)a.num_seqs * ((a.g + R - 1) / R);
+  // Tiles that have rows, as far as it is known here.
+  const int64_t full = a.row_indptr ? std::max<int64_t>(a.num_seqs, (int64_t)a.num_rows * a.g / R) : tiles;
+  int64_t pages = max_pages > 0 ? max_pages : INT64_MAX;
+  if (a.window > 0) pages = std::min(pages, ((int64_t)a.window + a.sinks) / kPageSize + 2);
+  const int nsplit = win_split(full * a.Hkv, (int64_t)sms * kWinCtas<D, KV, NT>, pages);
   const int64_t blocks = tiles * a.Hkv * nsplit;
   if (blocks > 0x7FFFFFFF) return fail(DD_ERR_INVALID_ARGUMENT, "too many rows");
   cudaError_t e = cudaSuccess;
@@ -657,17 +709,20 @@ static int launch_win_mma_t(const WinArgs& a, int64_t tiles, int nsplit, cudaStr
 }
 
 template <int D, int KV>
-static int launch_win_mma_nt(const WinArgs& a, int nt, int64_t tiles, int nsplit, cudaStream_t st) {
+static int launch_win_mma_nt(const WinArgs& a, int max_pages, int sms, cudaStream_t st) {
+  // Rows of an average sequence: one column block of 8 where they fit it, or
+  // where two of head_dim 256 would not fit the registers.
+  const int64_t rows = ((int64_t)a.num_rows * a.g + a.num_seqs - 1) / a.num_seqs;
   if constexpr (D < 256)
-    if (nt == 2) return launch_win_mma_t<D, KV, 2>(a, tiles, nsplit, st);
-  return launch_win_mma_t<D, KV, 1>(a, tiles, nsplit, st);
+    if (rows > 8) return launch_win_mma_t<D, KV, 2>(a, max_pages, sms, st);
+  return launch_win_mma_t<D, KV, 1>(a, max_pages, sms, st);
 }
 template <int D>
-static int launch_win_mma_kv(const WinArgs& a, int nt, int64_t tiles, int nsplit, cudaStream_t st) {
+static int launch_win_mma_kv(const WinArgs& a, int max_pages, int sms, cudaStream_t st) {
   switch (a.kv_dtype) {
-    case DD_DTYPE_BF16: return launch_win_mma_nt<D, kWinBf16>(a, nt, tiles, nsplit, st);
-    case DD_DTYPE_E4M3: return launch_win_mma_nt<D, kWinE4m3>(a, nt, tiles, nsplit, st);
-    default: return launch_win_mma_nt<D, kWinMx>(a, nt, tiles, nsplit, st);
+    case DD_DTYPE_BF16: return launch_win_mma_nt<D, kWinBf16>(a, max_pages, sms, st);
+    case DD_DTYPE_E4M3: return launch_win_mma_nt<D, kWinE4m3>(a, max_pages, sms, st);
+    default: return launch_win_mma_nt<D, kWinMx>(a, max_pages, sms, st);
   }
 }
 
@@ -675,24 +730,10 @@ static int launch_win_mma_kv(const WinArgs& a, int nt, int64_t tiles, int nsplit
 int launch_win_mma(const WinArgs& a, int max_pages, cudaStream_t st) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  // Rows of an average sequence: one column block of 8 where they fit it, or
-  // where two of head_dim 256 would not fit the registers.
-  const int64_t rows = std::max<int64_t>(1, ((int64_t)a.num_rows * a.g + a.num_seqs - 1) / a.num_seqs);
-  const int nt = rows <= 8 || a.D == 256 ? 1 : 2, R = 8 * nt;
-  const int64_t tiles = a.row_indptr ? a.num_seqs + (int64_t)a.num_rows * a.g / R
-                                     : (int64_t)a.num_seqs * ((a.g + R - 1) / R);
-  // Cluster size: about four CTAs for each of the three that an SM holds, so
-  // that unequal sequences even out, but at least two pages for each warp.
-  int64_t pages = max_pages > 0 ? max_pages : INT64_MAX;
-  if (a.window > 0) pages = std::min(pages, ((int64_t)a.window + a.sinks) / kPageSize + 2);
-  const int64_t units = std::max<int64_t>(1, (a.row_indptr ? std::max<int64_t>(1, (int64_t)a.num_rows * a.g / R) : tiles) * a.Hkv);
-  const int64_t want = std::min<int64_t>((12 * (int64_t)sms + units - 1) / units, pages / (2 * kWinWarps));
-  int nsplit = 1;
-  while (nsplit < 16 && nsplit < want) nsplit *= 2;
   switch (a.D) {
-    case 64: return launch_win_mma_kv<64>(a, nt, tiles, nsplit, st);
-    case 128: return launch_win_mma_kv<128>(a, nt, tiles, nsplit, st);
-    default: return launch_win_mma_kv<256>(a, nt, tiles, nsplit, st);
+    case 64: return launch_win_mma_kv<64>(a, max_pages, sms, st);
+    case 128: return launch_win_mma_kv<128>(a, max_pages, sms, st);
+    default: return launch_win_mma_kv<256>(a, max_pages, sms, st);
   }
 }
 
