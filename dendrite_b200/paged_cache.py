@@ -24,6 +24,21 @@ map). Here a step of B sequences (the leaves of a tree) is:
 Prompts go in through ``layer_prefill`` (the causal prefill plan of the new
 tokens over their sequence, ReferenceBackend::prefill's attention when the
 sequence starts empty).
+
+Layers whose tokens attend to a sliding window and a few first tokens are named
+in ``windows`` (``(window, sinks)`` per layer, None for full attention); they
+run without a plan, on device copies of the tables that ``begin_step`` makes,
+and never read the table entries of pages that no window reaches any more.
+
+A ragged batch of chunks (several sequences, any number of new tokens each,
+prompts in flight or tokens to be checked) goes in through
+
+* ``begin_chunks(tables, num_tokens, new_tokens)``: the batch, once for all
+  layers;
+* ``layer_chunk(layer, q, k, v)``: stores the layer's new K/V (quantised for
+  FP8 pools) and returns the causal attention, windowed or full;
+
+and ``read_tokens`` takes token ranges back out, dequantised.
 """
 from __future__ import annotations
 
@@ -33,6 +48,8 @@ import torch
 from . import _lib
 from .backend import (PAGE_SIZE, CascadePlan, _alloc_ws, append_kv_batch, cascade_decode,
                       make_config)
+from .paged_window import (append_kv_paged, decode_paged_window, gather_kv_paged,
+                           prefill_paged_window)
 
 _KV = {"bf16": _lib.DTYPE_BF16, "e4m3": _lib.DTYPE_E4M3, "mxfp8": _lib.DTYPE_MXFP8}
 
@@ -43,9 +60,13 @@ class PagedKVCache:
 
     def __init__(self, num_layers: int, num_pages: int, num_heads: int, num_kv_heads: int,
                  head_dim: int, kv_dtype: str = "bf16", e4m3_scales=None,
-                 device: str | torch.device = "cuda"):
+                 device: str | torch.device = "cuda", windows=None):
         if kv_dtype not in _KV:
             raise _lib.InvalidArgument("kv_dtype must be bf16, e4m3 or mxfp8")
+        self.windows = [None] * num_layers if windows is None else list(windows)
+        if len(self.windows) != num_layers or any(
+                w is not None and (len(w) != 2 or w[0] < 1 or w[1] < 0) for w in self.windows):
+            raise _lib.InvalidArgument("windows must be one (window >= 1, sinks >= 0) or None per layer")
         self.device = torch.device(device)
         self.Hq, self.Hkv, self.D, self.num_pages = num_heads, num_kv_heads, head_dim, num_pages
         self.kv_dtype = kv_dtype
@@ -72,6 +93,7 @@ class PagedKVCache:
         self._tables = None
         self._ws: dict = {}
         self._page_ids = self._slots = None
+        self._step = self._chunks = None  # device tables of the step / of the chunks
 
     # -- per step ---------------------------------------------------------
     def _only_grew(self, indptr, block_ids) -> bool:
@@ -96,6 +118,12 @@ class PagedKVCache:
         ntok = (pos + 1).astype(np.int32)
         blk = block_ids[indptr[:-1] + pos // PAGE_SIZE]
         advanced = False
+        if any(self.windows):
+            self._step = self._device_tables(indptr, block_ids, ntok)
+        self._page_ids = torch.from_numpy(blk.astype(np.int32)).to(self.device)
+        self._slots = torch.from_numpy((pos % PAGE_SIZE).astype(np.int32)).to(self.device)
+        if all(self.windows):  # nothing needs the plan
+            return advanced
         if self.plan is not None and self._ntok is not None and len(self._ntok) == len(ntok) \
                 and np.array_equal(self._ntok + 1, ntok) \
                 and (tree_grew_only or (tree_grew_only is None and self._only_grew(indptr, block_ids))):
@@ -108,15 +136,24 @@ class PagedKVCache:
         self.plan.upload(self.device)
         self._ntok = ntok
         self._tables = (indptr.copy(), block_ids.copy())
-        self._page_ids = torch.from_numpy(blk.astype(np.int32)).to(self.device)
-        self._slots = torch.from_numpy((pos % PAGE_SIZE).astype(np.int32)).to(self.device)
         return advanced
+
+    def _device_tables(self, indptr, block_ids, ntok):
+        """(page_indptr, page_indices, num_tokens on the device, pages of the longest table)."""
+        dev = [torch.from_numpy(np.ascontiguousarray(x).view(np.int32)).to(self.device)
+               for x in (indptr, block_ids, ntok)]
+        return (*dev, int(np.diff(indptr).max(initial=0)))
 
     def layer_step(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         """Store layer `layer`'s new K/V [B, Hkv, D] and attend with q [B, Hq, D]."""
         append_kv_batch(self.cfg, self.pools[layer], self.scales[layer], self._page_ids, self._slots,
                         k.contiguous(), v.contiguous())
         q = q.to(torch.bfloat16).contiguous()
+        if self.windows[layer]:
+            ip, ids, ntok, longest = self._step
+            out, _ = decode_paged_window(self.cfg, q, self.pools[layer], ip, ids, ntok, *self.windows[layer],
+                                         max_pages=longest, kv_scales=self.scales[layer])
+            return out
         ws = _alloc_ws(self.plan.info().workspace_bytes, self.device, self._ws)
         out, _ = cascade_decode(self.cfg, self.plan, q, self.pools[layer], self.scales[layer],
                                 workspace=ws)
@@ -130,6 +167,10 @@ class PagedKVCache:
         causal attention of q [S, Hq, D] (new token i sees tokens
         0 .. prefix_len + i)."""
         S = q.shape[0]
+        if self.windows[layer]:
+            tbl = np.asarray(table).astype(np.uint32)
+            self.begin_chunks([0, len(tbl)], tbl, [prefix_len + S], [S])
+            return self.layer_chunk(layer, q, k, v)
         pos = np.arange(prefix_len, prefix_len + S)
         tbl = np.asarray(table, dtype=np.uint32)
         page_ids = torch.from_numpy(tbl[pos // PAGE_SIZE].astype(np.int32)).to(self.device)
@@ -141,3 +182,47 @@ class PagedKVCache:
         out, _ = cascade_decode(self.cfg, plan, q.to(torch.bfloat16).contiguous(), self.pools[layer],
                                 self.scales[layer])
         return out
+
+    # -- chunks of several sequences ------------------------------------------
+    def begin_chunks(self, indptr, block_ids, num_tokens, new_tokens) -> None:
+        """A ragged batch: sequence s (table block_ids[indptr[s]:indptr[s + 1]])
+        will hold num_tokens[s] tokens, the last new_tokens[s] of them new."""
+        indptr = np.ascontiguousarray(indptr, dtype=np.int32)
+        ids = np.ascontiguousarray(np.asarray(block_ids).astype(np.uint32))
+        ntok = np.ascontiguousarray(num_tokens, dtype=np.int32)
+        new = np.ascontiguousarray(new_tokens, dtype=np.int32)
+        if len(indptr) != len(ntok) + 1 or len(new) != len(ntok) or np.any(np.diff(indptr) < 0) or \
+                np.any(new < 0) or np.any(new > ntok) or np.any(ntok > np.diff(indptr) * PAGE_SIZE) or \
+                indptr[-1] > len(ids):
+            raise _lib.InvalidArgument("tables, num_tokens and new_tokens do not fit together")
+        rows = np.concatenate([[0], np.cumsum(new, dtype=np.int64)]).astype(np.int32)
+        self._chunks = self._device_tables(indptr, ids, ntok) + (torch.from_numpy(rows).to(self.device),)
+
+    def layer_chunk(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """Store layer `layer`'s new K/V [rows, Hkv, D] of the batch of
+        begin_chunks and attend with q [rows, Hq, D] (rows sequence by
+        sequence; all three may be parts of a wider projection)."""
+        if self._chunks is None:
+            raise _lib.InvalidArgument("begin_chunks first")
+        ip, ids, ntok, longest, rows = self._chunks
+        append_kv_paged(self.cfg, self.pools[layer], self.scales[layer], rows, ip, ids, ntok, k, v)
+        window, sinks = self.windows[layer] or (0, 0)
+        out, _ = prefill_paged_window(self.cfg, q.to(torch.bfloat16), self.pools[layer], rows, ip, ids, ntok,
+                                      window, sinks, max_pages=longest, kv_scales=self.scales[layer])
+        return out
+
+    def read_tokens(self, layer: int, indptr, block_ids, first, count, out_dtype=torch.bfloat16):
+        """K and V [sum(count), Hkv, D] of tokens first[s] .. first[s] + count[s]
+        of each sequence, dequantised."""
+        indptr = np.ascontiguousarray(indptr, dtype=np.int32)
+        ids = np.ascontiguousarray(np.asarray(block_ids).astype(np.uint32))
+        first = np.ascontiguousarray(first, dtype=np.int32)
+        count = np.ascontiguousarray(count, dtype=np.int32)
+        if len(indptr) != len(first) + 1 or len(count) != len(first) or np.any(first < 0) or np.any(count < 0) or \
+                np.any(first.astype(np.int64) + count > np.diff(indptr).astype(np.int64) * PAGE_SIZE) or \
+                indptr[-1] > len(ids):
+            raise _lib.InvalidArgument("tables, first and count do not fit together")
+        ip, pages, start, _ = self._device_tables(indptr, ids, first)
+        rows = np.concatenate([[0], np.cumsum(count, dtype=np.int64)]).astype(np.int32)
+        return gather_kv_paged(self.cfg, self.pools[layer], self.scales[layer], torch.from_numpy(rows).to(self.device),
+                               start, ip, pages, int(rows[-1]), out_dtype)

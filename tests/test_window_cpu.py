@@ -205,3 +205,22 @@ def test_reference_codes_match_the_oracle():
     assert np.array_equal(c.numpy().reshape(-1), oc.reshape(-1)) and np.array_equal(e.numpy().reshape(-1), oe.reshape(-1))
     c, _ = encode(x, "e4m3", torch.tensor(0.017))
     assert np.array_equal(c.numpy(), oracle.e4m3_encode(x.numpy() / np.float32(0.017)))
+
+
+def test_paged_cache_refusals():
+    with pytest.raises(dd.InvalidArgument, match="windows"):
+        dd.PagedKVCache(2, 4, HQ, HKV, D, device="cpu", windows=[(4, 0)])
+    for bad in ((0, 1), (4, -1), (4,)):
+        with pytest.raises(dd.InvalidArgument, match="windows"):
+            dd.PagedKVCache(1, 4, HQ, HKV, D, device="cpu", windows=[bad])
+    cache = dd.PagedKVCache(1, 4, HQ, HKV, D, device="cpu", windows=[(4, 1)])
+    k = torch.zeros(1, HKV, D, dtype=torch.bfloat16)
+    with pytest.raises(dd.InvalidArgument, match="begin_chunks"):
+        cache.layer_chunk(0, torch.zeros(1, HQ, D, dtype=torch.bfloat16), k, k)
+    for args in (([0, 1], [0], [17], [1]), ([0, 1], [0], [3], [4]), ([0, 1], [0], [3, 3], [1, 1]), ([0, 2], [0], [3], [1]),
+                 ([0, 1], [0], [3], [-1])):
+        with pytest.raises(dd.InvalidArgument, match="fit together"):
+            cache.begin_chunks(*args)
+    for args in (([0, 1], [0], [10], [7]), ([0, 1], [0], [-1], [1]), ([0, 1], [0], [0], [-1]), ([0, 2], [0], [0], [1])):
+        with pytest.raises(dd.InvalidArgument, match="fit together"):
+            cache.read_tokens(0, *args)
