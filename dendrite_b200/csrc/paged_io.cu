@@ -46,17 +46,21 @@ __device__ __forceinline__ bool io_place(const PagedIo& a, int32_t row, bool rep
   return false;
 }
 
-// A warp owns a row: its K and V heads are one run of 2 * Hkv * D elements, cut
-// into 16-byte chunks of the pool's type (kN elements). A lane takes every 32nd
-// chunk, four at a time with all their loads ahead of the work, so the row's
-// place in the page table (a short chain of dependent reads) is paid once for
-// up to 2 KB of codes. Pool-side accesses are whole 128-byte runs of one head.
+// A row's K and V heads are one run of 2 * Hkv * D elements, cut into 16-byte
+// chunks of the pool's type (kN elements). A warp takes 32 chunks of a row, a
+// chunk a lane, or 128 in four rounds: the row's place in the page table is a
+// chain of dependent reads, which a small call pays as few times as it can in
+// turn (16 tokens: 2.7 us against 3.9) and a large one as few times as it can at
+// all (104,000 MXFP8 tokens read back: 122 us against 97, 6.1 TB/s; 32,000
+// tokens stored as E4M3 68 against 51, 4.0 TB/s, bound by its divisions' issue
+// slots beside HBM). Four chunks of a lane in flight cost registers, so warps,
+// and lost (119, 78). Pool-side accesses are
+// whole 128-byte runs of one head.
 template <int POOL>
 struct IoPool {
   static constexpr int kN = POOL == DD_DTYPE_F32 ? 4 : POOL == DD_DTYPE_BF16 ? 8 : 16;
 };
 constexpr int kIoWarps = 4;
-constexpr int kIoChunks = 4;  // chunks of a lane in flight
 
 // kN consecutive elements as f32, from / to 16-byte aligned (8 bytes for the
 // four bf16 of an f32 chunk) memory.
@@ -125,104 +129,95 @@ struct IoChunk {
   }
 };
 
-template <int POOL, int EXT>
+// Warp's row and its chunks [c0, c1), 32 times kRounds of them at most.
+template <int N, int kRounds>
+__device__ __forceinline__ bool io_share(const PagedIo& a, int32_t& row, int& c0, int& c1) {
+  const int64_t w = (int64_t)blockIdx.x * kIoWarps + (threadIdx.x >> 5);
+  const int all = 2 * (a.Hkv << a.log2_d) / N, parts = (all + 32 * kRounds - 1) / (32 * kRounds);
+  const int64_t r = parts == 1 ? w : w / parts;
+  if (r >= a.num_rows) return false;
+  row = (int32_t)r;
+  c0 = (int)(w - r * parts) * 32 * kRounds;
+  c1 = min(all, c0 + 32 * kRounds);
+  return true;
+}
+
+template <int POOL, int EXT, int kRounds>
 __global__ void __launch_bounds__(kIoWarps * 32) append_paged_kernel(PagedIo a) {
   constexpr int N = IoPool<POOL>::kN;
-  const int64_t w = (int64_t)blockIdx.x * kIoWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (w >= a.num_rows) return;
-  const int32_t row = (int32_t)w;
+  int32_t row;
+  int c0, c1;
+  if (!io_share<N, kRounds>(a, row, c0, c1)) return;
   uint32_t page;
   int32_t slot;
   bool live;
-  if (!io_place<true>(a, row, lane == 0, page, slot, live)) return;
+  if (!io_place<true>(a, row, c0 == 0 && lane == 0, page, slot, live)) return;
   const int half = (a.Hkv << a.log2_d) / N;
-  for (int c0 = lane; c0 - lane < 2 * half; c0 += 32 * kIoChunks) {
-    float x[kIoChunks][N];
 #pragma unroll
-    for (int u = 0; u < kIoChunks; ++u) {
-      const int c = c0 + 32 * u;
+  for (int u = 0; u < kRounds; ++u, c0 += 32) {
+    if (c0 >= c1) break;
+    const bool in = c0 + lane < c1;  // lanes past the end keep the warp's exchange whole
+    const IoChunk<N> k(a, in ? c0 + lane : 0, half, page, slot);
+    float x[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[u][i] = 0.f;
-      if (c < 2 * half) {
-        const IoChunk<N> k(a, c, half, page, slot);
-        io_load<EXT, N>(k.which ? a.v : a.k, (int64_t)row * (k.which ? a.v_stride : a.k_stride) + k.ext, x[u]);
-      }
-    }
+    for (int i = 0; i < N; ++i) x[i] = 0.f;
+    if (in) io_load<EXT, N>(k.which ? a.v : a.k, (int64_t)row * (k.which ? a.v_stride : a.k_stride) + k.ext, x);
+    const int64_t dst = (k.row << a.log2_d) + k.d;
+    if constexpr (POOL == DD_DTYPE_F32 || POOL == DD_DTYPE_BF16) {
+      if (in) io_store<POOL, N>(a.kv, dst, x);
+    } else {
+      if constexpr (POOL == DD_DTYPE_E4M3) {
+        const float sc = reinterpret_cast<const float*>(a.scales)[k.which * a.Hkv + k.h];
 #pragma unroll
-    for (int u = 0; u < kIoChunks; ++u) {
-      const int c = c0 + 32 * u;
-      const bool in = c < 2 * half;
-      const IoChunk<N> k(a, in ? c : 0, half, page, slot);
-      const int64_t dst = (k.row << a.log2_d) + k.d;
-      if constexpr (POOL == DD_DTYPE_F32 || POOL == DD_DTYPE_BF16) {
-        if (in) io_store<POOL, N>(a.kv, dst, x[u]);
+        for (int i = 0; i < N; ++i) x[i] = __fdiv_rn(x[i], sc);
       } else {
-        if constexpr (POOL == DD_DTYPE_E4M3) {
-          const float sc = reinterpret_cast<const float*>(a.scales)[k.which * a.Hkv + k.h];
+        // 32 elements are two neighbouring lanes' chunks.
+        float m = 0.f;
 #pragma unroll
-          for (int i = 0; i < N; ++i) x[u][i] = __fdiv_rn(x[u][i], sc);
-        } else {
-          // 32 elements are two neighbouring lanes' chunks.
-          float m = 0.f;
+        for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[i]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        const int ex = m > 0.f ? max(floor_log2_pos(m) - 8, -127) : -127;
+        const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);  // 2^-ex, a normal f32
 #pragma unroll
-          for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(x[u][i]));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          const int ex = m > 0.f ? max(floor_log2_pos(m) - 8, -127) : -127;
-          const float inv = __uint_as_float((uint32_t)(127 - ex) << 23);  // 2^-ex, a normal f32
-#pragma unroll
-          for (int i = 0; i < N; ++i) x[u][i] *= inv;
-          if (in && !(lane & 1))
-            reinterpret_cast<uint8_t*>(a.scales)[(k.row << (a.log2_d - 5)) + (k.d >> 5)] = (uint8_t)(ex + 127);
-        }
-        uint32_t q[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          q[i] = e4m3x4_satrn(x[u][4 * i], x[u][4 * i + 1], x[u][4 * i + 2], x[u][4 * i + 3]);
-        if (in) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.kv) + dst) = make_uint4(q[0], q[1], q[2], q[3]);
+        for (int i = 0; i < N; ++i) x[i] *= inv;
+        if (in && !(lane & 1))
+          reinterpret_cast<uint8_t*>(a.scales)[(k.row << (a.log2_d - 5)) + (k.d >> 5)] = (uint8_t)(ex + 127);
       }
+      uint32_t q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[i] = e4m3x4_satrn(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+      if (in) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(a.kv) + dst) = make_uint4(q[0], q[1], q[2], q[3]);
     }
   }
 }
 
-template <int POOL, int EXT>
+template <int POOL, int EXT, int kRounds>
 __global__ void __launch_bounds__(kIoWarps * 32) gather_paged_kernel(PagedIo a) {
   constexpr int N = IoPool<POOL>::kN;
-  const int64_t w = (int64_t)blockIdx.x * kIoWarps + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  if (w >= a.num_rows) return;
-  const int32_t row = (int32_t)w;
+  int32_t row;
+  int c0, c1;
+  if (!io_share<N, kRounds>(a, row, c0, c1)) return;
   uint32_t page;
   int32_t slot;
   bool live;
-  const bool ok = io_place<false>(a, row, lane == 0, page, slot, live);
+  const bool ok = io_place<false>(a, row, c0 == 0 && lane == 0, page, slot, live);
   if (!live) return;
   const int half = (a.Hkv << a.log2_d) / N;
   const int64_t width = (int64_t)a.Hkv << a.log2_d;
-  for (int c0 = lane; c0 < 2 * half; c0 += 32 * kIoChunks) {
-    uint4 v[kIoChunks];
-    float sc[kIoChunks];
 #pragma unroll
-    for (int u = 0; u < kIoChunks; ++u) {
-      const int c = c0 + 32 * u;
-      v[u] = make_uint4(0, 0, 0, 0);
-      sc[u] = 1.f;
-      if (ok && c < 2 * half) {
-        const IoChunk<N> k(a, c, half, page, slot);
-        v[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.kv) +
-                                               ((k.row << a.log2_d) + k.d) * (16 / N));
-        if constexpr (POOL == DD_DTYPE_E4M3) sc[u] = reinterpret_cast<const float*>(a.scales)[k.which * a.Hkv + k.h];
-        if constexpr (POOL == DD_DTYPE_MXFP8)
-          sc[u] = e8m0_to_float(reinterpret_cast<const uint8_t*>(a.scales)[(k.row << (a.log2_d - 5)) + (k.d >> 5)]);
-      }
-    }
+  for (int u = 0; u < kRounds; ++u) {
+    const int c = c0 + lane + 32 * u;
+    if (c >= c1) break;
+    const IoChunk<N> k(a, c, half, ok ? page : 0, slot);
+    float x[N];
 #pragma unroll
-    for (int u = 0; u < kIoChunks; ++u) {
-      const int c = c0 + 32 * u;
-      if (c >= 2 * half) break;
-      const IoChunk<N> k(a, c, half, 0, 0);
-      const uint32_t q[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-      float x[N];
+    for (int i = 0; i < N; ++i) x[i] = 0.f;
+    if (ok) {
+      const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(a.kv) +
+                                                      ((k.row << a.log2_d) + k.d) * (16 / N));
+      const uint32_t q[4] = {v.x, v.y, v.z, v.w};
       if constexpr (POOL == DD_DTYPE_F32) {
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = __uint_as_float(q[i]);
@@ -233,40 +228,53 @@ __global__ void __launch_bounds__(kIoWarps * 32) gather_paged_kernel(PagedIo a) 
           x[2 * i + 1] = __uint_as_float(q[i] & 0xffff0000u);
         }
       } else {
+        const float sc = POOL == DD_DTYPE_E4M3
+                             ? reinterpret_cast<const float*>(a.scales)[k.which * a.Hkv + k.h]
+                             : e8m0_to_float(reinterpret_cast<const uint8_t*>(
+                                   a.scales)[(k.row << (a.log2_d - 5)) + (k.d >> 5)]);
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
           const float2 y = e4m3x2_to_float2((uint16_t)(i & 1 ? q[i / 2] >> 16 : q[i / 2] & 0xffffu));
-          x[2 * i] = y.x * sc[u];
-          x[2 * i + 1] = y.y * sc[u];
+          x[2 * i] = y.x * sc;
+          x[2 * i + 1] = y.y * sc;
         }
       }
-      io_store<EXT, N>(const_cast<void*>(k.which ? a.v : a.k), (int64_t)row * width + k.ext, x);
     }
+    io_store<EXT, N>(const_cast<void*>(k.which ? a.v : a.k), (int64_t)row * width + k.ext, x);
   }
 }
 
-template <int POOL>
-static void launch_io(bool append, const PagedIo& a, cudaStream_t st) {
-  const unsigned blocks = (unsigned)(((int64_t)a.num_rows + kIoWarps - 1) / kIoWarps);
+template <int POOL, int EXT, int kRounds>
+static void launch_io_t(bool append, const PagedIo& a, cudaStream_t st) {
+  const int64_t all = 2 * ((int64_t)a.Hkv << a.log2_d) / IoPool<POOL>::kN;
+  const int64_t parts = (all + 32 * kRounds - 1) / (32 * kRounds);
+  const unsigned blocks = (unsigned)((a.num_rows * parts + kIoWarps - 1) / kIoWarps);
   ProfScope ps(kProfOther, st);
-  if (append) {
-    if (a.ext_dtype == DD_DTYPE_F32)
-      append_paged_kernel<POOL, DD_DTYPE_F32><<<blocks, kIoWarps * 32, 0, st>>>(a);
-    else
-      append_paged_kernel<POOL, DD_DTYPE_BF16><<<blocks, kIoWarps * 32, 0, st>>>(a);
-  } else {
-    if (a.ext_dtype == DD_DTYPE_F32)
-      gather_paged_kernel<POOL, DD_DTYPE_F32><<<blocks, kIoWarps * 32, 0, st>>>(a);
-    else
-      gather_paged_kernel<POOL, DD_DTYPE_BF16><<<blocks, kIoWarps * 32, 0, st>>>(a);
-  }
+  if (append)
+    append_paged_kernel<POOL, EXT, kRounds><<<blocks, kIoWarps * 32, 0, st>>>(a);
+  else
+    gather_paged_kernel<POOL, EXT, kRounds><<<blocks, kIoWarps * 32, 0, st>>>(a);
+}
+template <int POOL>
+static void launch_io(bool append, const PagedIo& a, int sms, cudaStream_t st) {
+  const int64_t all = 2 * ((int64_t)a.Hkv << a.log2_d) / IoPool<POOL>::kN;
+  // One round a warp as long as these warps fit the GPU at once.
+  const bool one = a.num_rows * ((all + 31) / 32) <= (int64_t)sms * 32;
+  const bool f32 = a.ext_dtype == DD_DTYPE_F32;
+  if (one)
+    f32 ? launch_io_t<POOL, DD_DTYPE_F32, 1>(append, a, st) : launch_io_t<POOL, DD_DTYPE_BF16, 1>(append, a, st);
+  else
+    f32 ? launch_io_t<POOL, DD_DTYPE_F32, 4>(append, a, st) : launch_io_t<POOL, DD_DTYPE_BF16, 4>(append, a, st);
 }
 static int run_io(bool append, const PagedIo& a, cudaStream_t st) {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if ((int64_t)a.num_rows * a.Hkv > (1ll << 31)) return fail(DD_ERR_INVALID_ARGUMENT, "too many rows");
   switch (a.pool_dtype) {
-    case DD_DTYPE_F32: launch_io<DD_DTYPE_F32>(append, a, st); break;
-    case DD_DTYPE_BF16: launch_io<DD_DTYPE_BF16>(append, a, st); break;
-    case DD_DTYPE_E4M3: launch_io<DD_DTYPE_E4M3>(append, a, st); break;
-    default: launch_io<DD_DTYPE_MXFP8>(append, a, st); break;
+    case DD_DTYPE_F32: launch_io<DD_DTYPE_F32>(append, a, sms, st); break;
+    case DD_DTYPE_BF16: launch_io<DD_DTYPE_BF16>(append, a, sms, st); break;
+    case DD_DTYPE_E4M3: launch_io<DD_DTYPE_E4M3>(append, a, sms, st); break;
+    default: launch_io<DD_DTYPE_MXFP8>(append, a, sms, st); break;
   }
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess)

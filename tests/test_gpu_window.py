@@ -398,3 +398,35 @@ def test_append_one_token_per_sequence(cuda):
     for page, slot, x in ((0, 0, 1), (1, 3, 2), (3, 15, 3)):
         assert pool[page, 0, :, slot].eq(x).all() and pool[page, 1, :, slot].eq(-x).all()
     assert pool.float().abs().sum().item() == 2 * Hkv * D * 6
+
+
+def test_append_e4m3_at_the_borders_of_codes(cuda):
+    """x / scale rounded to f32 and then to E4M3: x within a few steps of every
+    border between two codes, and where the quotient leaves f32's middle range,
+    under scales of all kinds. The codes are those of torch's f32 division."""
+    Hkv, D = 1, 256
+    codes = torch.arange(0, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()
+    borders = torch.cat([(codes[1:] + codes[:-1]) / 2, codes, torch.tensor([464.0, 480.0, 1e3, 2.0 ** -21, 2.0 ** 11])])
+    g = torch.Generator().manual_seed(9)
+    scales = torch.cat([torch.rand(20, generator=g) * 0.1, torch.exp2(torch.randint(-60, 60, (12,), generator=g).float()),
+                        torch.rand(12, generator=g) * 2.0 ** -60, torch.tensor([1.0, 2.0 ** -70, 2.0 ** 80, 2.0 ** -126])])
+    scales = torch.where(scales > 0, scales, torch.tensor(1.0)).float()
+    cfg = dd.make_config(Hkv, Hkv, D, 8, kv_dtype=KVD["e4m3"])
+    for s in scales:
+        x = (borders * s.double()).float()
+        ulp = torch.nextafter(x, torch.tensor(float("inf"))) - x
+        x = torch.cat([x + i * ulp for i in range(-4, 5)])
+        x = torch.cat([x, -x, torch.tensor([0.0, -0.0, float("inf"), -float("inf"), 1e-40, -1e-40, 3e38, float("nan")])])
+        rows = -(-x.numel() // D)
+        x = torch.cat([x, torch.zeros(rows * D - x.numel())]).view(rows, Hkv, D)
+        assert rows <= 16 * 8
+        pool = torch.zeros(8, 2, Hkv, PAGE, D, dtype=torch.uint8, device=cuda)
+        sc = torch.stack([s, s]).view(2, 1).to(cuda)
+        dd.append_kv_paged(cfg, pool, sc, _ints([0, rows], cuda), _ints([0, 8], cuda), _ints(list(range(8)), cuda),
+                           _ints([rows], cuda), x.to(cuda), x.to(cuda))
+        q = x / s
+        want = torch.where(q.isnan(), torch.tensor(0x7F, dtype=torch.uint8), encode(x, "e4m3", s)[0])
+        for which in (0, 1):
+            got = pool[:, which].permute(0, 2, 1, 3).reshape(-1, Hkv, D)[:rows].cpu()
+            ok = (got == want) | (q.isnan() & (got & 0x7F == 0x7F))
+            assert ok.all(), (s.item(), x[~ok][:4], got[~ok][:4], want[~ok][:4])
