@@ -51,7 +51,7 @@ __device__ __forceinline__ bool io_place(const PagedIo& a, int32_t row, bool rep
 // chunk a lane, or 128 in four rounds: the row's place in the page table is a
 // chain of dependent reads, which a small call pays as few times as it can in
 // turn (16 tokens: 2.7 us against 3.9) and a large one as few times as it can at
-// all (104,000 MXFP8 tokens read back: 122 us against 97, 6.1 TB/s; 32,000
+// all (95,000 MXFP8 tokens read back: 122 us against 97, 6.1 TB/s; 33,000
 // tokens stored as E4M3 68 against 51, 4.0 TB/s, bound by its divisions' issue
 // slots beside HBM). Four chunks of a lane in flight cost registers, so warps,
 // and lost (119, 78). Pool-side accesses are
