@@ -269,7 +269,7 @@ static void launch_io(bool append, const PagedIo& a, int sms, cudaStream_t st) {
 static int run_io(bool append, const PagedIo& a, cudaStream_t st) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if ((int64_t)a.num_rows * a.Hkv > (1ll << 31)) return fail(DD_ERR_INVALID_ARGUMENT, "too many rows");
+  if ((int64_t)a.num_rows * a.Hkv >= (1ll << 31)) return fail(DD_ERR_INVALID_ARGUMENT, "too many rows");
   switch (a.pool_dtype) {
     case DD_DTYPE_F32: launch_io<DD_DTYPE_F32>(append, a, sms, st); break;
     case DD_DTYPE_BF16: launch_io<DD_DTYPE_BF16>(append, a, sms, st); break;

@@ -140,6 +140,8 @@ class PagedKVCache:
 
     def _device_tables(self, indptr, block_ids, ntok):
         """(page_indptr, page_indices, num_tokens on the device, pages of the longest table)."""
+        if indptr[0] < 0 or np.any(np.diff(indptr) < 0) or indptr[-1] > len(block_ids):
+            raise _lib.InvalidArgument("the tables and the block ids do not fit together")
         dev = [torch.from_numpy(np.ascontiguousarray(x).view(np.int32)).to(self.device)
                for x in (indptr, block_ids, ntok)]
         return (*dev, int(np.diff(indptr).max(initial=0)))
@@ -169,8 +171,7 @@ class PagedKVCache:
         S = q.shape[0]
         if self.windows[layer]:
             tbl = np.asarray(table).astype(np.uint32)
-            self.begin_chunks([0, len(tbl)], tbl, [prefix_len + S], [S])
-            return self.layer_chunk(layer, q, k, v)
+            return self._chunk(layer, self._chunk_tables([0, len(tbl)], tbl, [prefix_len + S], [S]), q, k, v)
         pos = np.arange(prefix_len, prefix_len + S)
         tbl = np.asarray(table, dtype=np.uint32)
         page_ids = torch.from_numpy(tbl[pos // PAGE_SIZE].astype(np.int32)).to(self.device)
@@ -187,27 +188,36 @@ class PagedKVCache:
     def begin_chunks(self, indptr, block_ids, num_tokens, new_tokens) -> None:
         """A ragged batch: sequence s (table block_ids[indptr[s]:indptr[s + 1]])
         will hold num_tokens[s] tokens, the last new_tokens[s] of them new."""
+        self._chunks = self._chunk_tables(indptr, block_ids, num_tokens, new_tokens)
+
+    def _chunk_tables(self, indptr, block_ids, num_tokens, new_tokens):
+        """_device_tables of a ragged batch, its rows' borders on the device, and its rows."""
         indptr = np.ascontiguousarray(indptr, dtype=np.int32)
         ids = np.ascontiguousarray(np.asarray(block_ids).astype(np.uint32))
         ntok = np.ascontiguousarray(num_tokens, dtype=np.int32)
         new = np.ascontiguousarray(new_tokens, dtype=np.int32)
-        if len(indptr) != len(ntok) + 1 or len(new) != len(ntok) or np.any(np.diff(indptr) < 0) or \
-                np.any(new < 0) or np.any(new > ntok) or np.any(ntok > np.diff(indptr) * PAGE_SIZE) or \
-                indptr[-1] > len(ids):
+        if len(indptr) != len(ntok) + 1 or len(new) != len(ntok) or np.any(new < 0) or np.any(new > ntok) or \
+                np.any(ntok > np.diff(indptr).astype(np.int64) * PAGE_SIZE):
             raise _lib.InvalidArgument("tables, num_tokens and new_tokens do not fit together")
         rows = np.concatenate([[0], np.cumsum(new, dtype=np.int64)]).astype(np.int32)
-        self._chunks = self._device_tables(indptr, ids, ntok) + (torch.from_numpy(rows).to(self.device),)
+        return self._device_tables(indptr, ids, ntok) + (torch.from_numpy(rows).to(self.device), int(rows[-1]))
 
     def layer_chunk(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         """Store layer `layer`'s new K/V [rows, Hkv, D] of the batch of
         begin_chunks and attend with q [rows, Hq, D] (rows sequence by
-        sequence; all three may be parts of a wider projection)."""
+        sequence; all three may be parts of a wider projection, and have more
+        rows than the batch, whose outputs then are not set)."""
         if self._chunks is None:
             raise _lib.InvalidArgument("begin_chunks first")
-        ip, ids, ntok, longest, rows = self._chunks
-        append_kv_paged(self.cfg, self.pools[layer], self.scales[layer], rows, ip, ids, ntok, k, v)
+        return self._chunk(layer, self._chunks, q, k, v)
+
+    def _chunk(self, layer, tables, q, k, v):
+        ip, ids, ntok, longest, borders, rows = tables
+        if not q.shape[0] == k.shape[0] == v.shape[0] >= rows:
+            raise _lib.InvalidArgument(f"q, k and v must have the batch's {rows} rows")
+        append_kv_paged(self.cfg, self.pools[layer], self.scales[layer], borders, ip, ids, ntok, k, v)
         window, sinks = self.windows[layer] or (0, 0)
-        out, _ = prefill_paged_window(self.cfg, q.to(torch.bfloat16), self.pools[layer], rows, ip, ids, ntok,
+        out, _ = prefill_paged_window(self.cfg, q.to(torch.bfloat16), self.pools[layer], borders, ip, ids, ntok,
                                       window, sinks, max_pages=longest, kv_scales=self.scales[layer])
         return out
 
@@ -219,8 +229,7 @@ class PagedKVCache:
         first = np.ascontiguousarray(first, dtype=np.int32)
         count = np.ascontiguousarray(count, dtype=np.int32)
         if len(indptr) != len(first) + 1 or len(count) != len(first) or np.any(first < 0) or np.any(count < 0) or \
-                np.any(first.astype(np.int64) + count > np.diff(indptr).astype(np.int64) * PAGE_SIZE) or \
-                indptr[-1] > len(ids):
+                np.any(first.astype(np.int64) + count > np.diff(indptr).astype(np.int64) * PAGE_SIZE):
             raise _lib.InvalidArgument("tables, first and count do not fit together")
         ip, pages, start, _ = self._device_tables(indptr, ids, first)
         rows = np.concatenate([[0], np.cumsum(count, dtype=np.int64)]).astype(np.int32)

@@ -90,6 +90,8 @@ def _call(dev: int, fn, name: str, args, stream) -> None:
 
 def _attend(cfg, q, kv_pages, q_indptr, page_indptr, page_indices, num_tokens, window, sinks, max_pages,
             kv_scales, out, lse, status, stream):
+    if not (0 <= window < 1 << 31 and 0 <= sinks < 1 << 31 and 0 <= max_pages < 1 << 31):
+        _fail("window, sinks and max_pages must be >= 0 and below 2^31")  # ctypes would cut them off
     heads, dim = cfg.num_qo_heads, cfg.head_dim
     stride = _check_rows("q", q, heads, dim)
     if q.dtype != (torch.float32 if cfg.q_dtype == DTYPE_F32 else torch.bfloat16):
@@ -196,8 +198,8 @@ def gather_kv_paged(cfg: AttnConfig, kv_pages: torch.Tensor, kv_scales: torch.Te
     _check_pool(cfg, kv_pages, kv_scales)
     if out_dtype not in (torch.bfloat16, torch.float32):
         _fail("out_dtype must be bf16 or f32")
-    if num_rows < 0:
-        _fail("num_rows must be >= 0")
+    if not 0 <= num_rows < 1 << 31:
+        _fail("num_rows must be >= 0 and below 2^31")
     _check_index("out_indptr", out_indptr, 1)
     seqs = out_indptr.numel() - 1
     _check_index("page_indptr", page_indptr, seqs + 1)

@@ -331,6 +331,7 @@ int dd_decode_paged_static_status(dd_stream_t stream, uint32_t* code, uint32_t* 
  * a fused projection's output can be taken in place; 16-byte aligned).
  * out: [rows][num_qo_heads][head_dim], dense, 16-byte aligned. lse as above
  * (may be NULL). Rows at or past q_indptr[num_seqs] are left as they are.
+ * The outputs may not overlap the inputs.
  * max_pages_per_seq (0: not known) only guides how the work is divided.
  * No workspace; one kernel per call; calls on different streams are
  * independent. bf16 queries over bf16 / E4M3 / MXFP8 pages run on the tensor

@@ -224,3 +224,34 @@ def test_paged_cache_refusals():
     for args in (([0, 1], [0], [10], [7]), ([0, 1], [0], [-1], [1]), ([0, 1], [0], [0], [-1]), ([0, 2], [0], [0], [1])):
         with pytest.raises(dd.InvalidArgument, match="fit together"):
             cache.read_tokens(0, *args)
+
+
+@pytest.mark.parametrize("kw", [dict(window=1 << 31), dict(window=1 << 32), dict(window=-1), dict(sinks=1 << 32),
+                                dict(sinks=-1), dict(max_pages=1 << 32), dict(max_pages=-1)], ids=str)
+def test_sizes_that_32_bits_do_not_hold(kw):
+    cfg, a = _args(**kw)
+    with pytest.raises(dd.InvalidArgument, match="2.31"):
+        dd.prefill_paged_window(cfg, **a)
+    a.pop("q_indptr")
+    with pytest.raises(dd.InvalidArgument, match="2.31"):
+        dd.decode_paged_window(cfg, **a)
+
+
+def test_paged_cache_tables_that_reach_outside():
+    cache = dd.PagedKVCache(1, 4, HQ, HKV, D, device="cpu", windows=[(4, 1)])
+    for indptr in ([-1, 0], [0, 2, 1], [0, 1, 3]):
+        n = len(indptr) - 1
+        with pytest.raises(dd.InvalidArgument, match="fit together"):
+            cache.begin_chunks(indptr, [0, 1], [0] * n, [0] * n)
+        with pytest.raises(dd.InvalidArgument, match="fit together"):
+            cache.read_tokens(0, indptr, [0, 1], [0] * n, [0] * n)
+
+
+def test_paged_cache_chunks_need_their_rows():
+    cache = dd.PagedKVCache(1, 4, HQ, HKV, D, device="cpu", windows=[(4, 1)])
+    cache.begin_chunks([0, 1], [0], [5], [5])
+    def rows(n, heads):
+        return torch.zeros(n, heads, D, dtype=torch.bfloat16)
+    for nq, nk in ((4, 4), (5, 4), (4, 5), (6, 5)):
+        with pytest.raises(dd.InvalidArgument, match="5 rows"):
+            cache.layer_chunk(0, rows(nq, HQ), rows(nk, HKV), rows(nk, HKV))
