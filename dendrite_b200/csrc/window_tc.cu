@@ -41,6 +41,7 @@
 // masked; V of slots that no row of the item sees is zeroed before the product
 // (zero times NaN is not zero).
 #include <algorithm>
+#include <cfloat>
 
 #include "tc_common.cuh"
 #include "window.cuh"
@@ -220,7 +221,7 @@ __device__ __forceinline__ void prefetch_tma_4d(const CUtensorMap* map, int32_t 
 
 // 64 bytes of this thread's row of out: whole 32-byte sectors at a time where
 // the address allows (16 bytes at a time are twice the requests, and the rows
-// of a warp are as many lines apart: 6700 against 4400 cycles an item).
+// of a warp are as many lines apart).
 __device__ __forceinline__ void store16(uint16_t* out, const uint32_t (&w)[16], bool wide) {
   if (wide) {
 #pragma unroll
@@ -392,7 +393,9 @@ __global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
       const WtItem cur = it;
       const bool active = is_active(cur);
       if constexpr (kF16) {
-        scale_log2 = f16_score_scale(a.scale_log2, up) * reinterpret_cast<const float*>(a.scales)[cur.h];
+        // Above zero, which would make NaN of the -inf of a masked score (the
+        // scores of a row of zeros, whose power of two is the largest, stay zero).
+        scale_log2 = fmaxf(f16_score_scale(a.scale_log2, up) * reinterpret_cast<const float*>(a.scales)[cur.h], FLT_MIN);
         v_scale = reinterpret_cast<const float*>(a.scales)[a.Hkv + cur.h];
       }
       const int32_t p = cur.p_lo + tok;
