@@ -64,6 +64,14 @@ struct WtCfg {
   static constexpr int kExps = kTcTok * (D / 32);        // MXFP8 exponents of a tile
   static constexpr int kProducer = kFp8 ? 12 : 8;        // then two issuers and the scheduler
   static constexpr int kThreads = 32 * (kProducer + 4);
+  // FP8: the softmax takes registers over from the other warps and holds a
+  // tile's scores, in place of reading their first half again (8 chunks of 200
+  // to 700 tokens, window 1024, MXFP8: 96 us -> 92; 4 of 1000, window 2048,
+  // E4M3: 309 -> 306; bf16, 8191 tokens, window 4096: 384 -> 391, so not there).
+  // Together no more than the block's at launch.
+  static constexpr bool kHeld = kFp8;
+  static constexpr int kRegs = kFp8 ? 128 : 168, kRegsSoftmax = 184, kRegsConvert = 80, kRegsRest = 64;
+  static_assert(256 * kRegsSoftmax + 128 * kRegsConvert + 128 * kRegsRest <= 512 * 128);
   static constexpr int kSmem = (2 + kSlots) * kTileBytes + (kFp8 ? kWtStages * (kCodes + kExps) : 0) + 1024;
   // D f32, M = 128; A / B type in bits 7 and 10 (0 f16, 1 bf16); N in bits 17-22.
   static constexpr uint32_t kType = kF16 ? 0u : (1u << 7) | (1u << 10);
@@ -267,11 +275,11 @@ __device__ __forceinline__ void wt_weights(const float (&s)[32], uint64_t sc2, u
 }
 
 template <int D, int KV>
-__global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
+__global__ void __maxnreg__((WtCfg<D, KV>::kRegs))
     win_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, WinArgs a,
                   int32_t units) {
   using Cfg = WtCfg<D, KV>;
-  constexpr bool kFp8 = Cfg::kFp8, kF16 = Cfg::kF16;
+  constexpr bool kFp8 = Cfg::kFp8, kF16 = Cfg::kF16, kHeld = Cfg::kHeld;
   constexpr int kSlots = Cfg::kSlots, kTile = Cfg::kTileBytes, kHalf = Cfg::kHalfBytes;
   extern __shared__ uint8_t smem_raw[];
   __shared__ WtBars bars;
@@ -343,6 +351,7 @@ __global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
 
   if (warp < 8) {
     // ----------------------------------------------------------------- softmax
+    if constexpr (kHeld) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsSoftmax) : "memory");
     const int x = warp >> 2;        // sub-tile
     const int quarter = warp & 3;   // TMEM lanes [32 * quarter, + 32)
     const int r = quarter * 32 + lane;
@@ -413,12 +422,16 @@ __global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
         const uint32_t pages = __ballot_sync(0xffffffffu, entry < (uint32_t)a.num_pages) & 0xffu;
         entry = wt_entry(a, cur, (c / 2 + 1) * kTcPagesPerTile + pj);
         const bool seen_whole = wt_whole(a, cur, x0, kTcTok), whole = pages == 0xffu && seen_whole;
-        float s[2][32];
+        float s[kHeld ? 4 : 2][32];
         // Scores of half h, those that the row does not see as -inf.
         auto load = [&](int h) {
-          tmem_ld32(s_col + kWtChunk * h, s[0]);
-          tmem_ld32(s_col + kWtChunk * h + 32, s[1]);
-          tmem_wait_ld();
+          float(*sh)[32] = s + (kHeld ? 2 * h : 0);
+          tmem_ld32(s_col + kWtChunk * h, sh[0]);
+          tmem_ld32(s_col + kWtChunk * h + 32, sh[1]);
+          if (!kHeld || h == 1 || !two) tmem_wait_ld();
+        };
+        auto mask = [&](int h) {
+          float(*sh)[32] = s + (kHeld ? 2 * h : 0);
           if (whole) return;
           auto below = [](int32_t n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
 #pragma unroll
@@ -429,16 +442,17 @@ __global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
             if (!((pages >> (4 * h + 2 * i + 1)) & 1)) see &= 0x0000ffffu;
 #pragma unroll
             for (int k = 0; k < 32; ++k)
-              if (!((see >> k) & 1)) s[i][k] = -INFINITY;
+              if (!((see >> k) & 1)) sh[i][k] = -INFINITY;
           }
         };
         // (A NaN or infinite score passes the maximum by or makes it infinite;
         // its exponential is NaN either way, and with it the row's sum.)
-        auto row_max = [&]() {
+        auto row_max = [&](int h) {
+          const float(*sh)[32] = s + (kHeld ? 2 * h : 0);
           float mx[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float* v = &s[i / 2][16 * (i % 2)];
+            const float* v = &sh[i / 2][16 * (i % 2)];
             mx[i] = fmaxf(v[0], v[1]);
 #pragma unroll
             for (int k = 2; k < 16; k += 2) mx[i] = max3f(mx[i], v[k], v[k + 1]);
@@ -449,10 +463,13 @@ __global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
         ++tiles;
         tc_fence_after();
         load(0);
-        float mt = row_max();
+        if (kHeld && two) load(1);
+        mask(0);
+        float mt = row_max(0);
         if (two) {
-          load(1);
-          mt = fmaxf(mt, row_max());
+          if (!kHeld) load(1);
+          mask(1);
+          mt = fmaxf(mt, row_max(1));
         }
         mt = ok ? mt * scale_log2 : m_used;
         if (__any_sync(0xffffffffu, mt > m_used + Cfg::kStep)) {
@@ -479,15 +496,19 @@ __global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
         const float ref = (m_used == -INFINITY ? 0.f : m_used) - Cfg::kShift;
         const uint64_t nm2 = f2_pack(-ref, -ref);
         auto hand_over = [&](int h) {
-          wt_weights<kF16>(s[0], sc2, nm2, lsum, s_col + kWtChunk * h);
-          wt_weights<kF16>(s[1], sc2, nm2, lsum, s_col + kWtChunk * h + 16);
+          float(*sh)[32] = s + (kHeld ? 2 * h : 0);
+          wt_weights<kF16>(sh[0], sc2, nm2, lsum, s_col + kWtChunk * h);
+          wt_weights<kF16>(sh[1], sc2, nm2, lsum, s_col + kWtChunk * h + 16);
           tmem_wait_st();
           tc_fence_before();
           warp_arrive(&bars.p_full[x][h]);
         };
         if (two) {
           hand_over(1);
-          load(0);  // again: 64 registers hold a half at a time
+          if (!kHeld) {  // again
+            load(0);
+            mask(0);
+          }
         }
         hand_over(0);
       }
@@ -534,6 +555,7 @@ __global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
     }
   } else if (kFp8 && warp < 12) {
     // -------------------------------------------------------------- converters
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsConvert) : "memory");
     // A thread widens 16 codes of one token at a time; eight neighbouring
     // threads cover two rows, so their stores fall into eight bank groups.
     const int t = threadIdx.x - 256;
@@ -597,189 +619,192 @@ __global__ void __launch_bounds__(WtCfg<D, KV>::kThreads, 1)
         if (lane == 0) mbar_arrive(&bars.st_empty[su]);
       }
     }
-  } else if (warp == Cfg::kProducer) {
-    // ---------------------------------------------------------------- producer
-    const int64_t rows_total = (int64_t)a.num_pages * 2 * a.Hkv * kPageSize;
-    const int pj = lane & (kTcPagesPerTile - 1);
-    const bool mine = lane < kTcPagesPerTile;
-    int gidx = 0;
-    bool ok = true;
-    while (ok && next_item(it)) {
-      uint32_t cur = wt_entry(a, it, pj), nxt = 0xFFFFFFFFu;
-      const int ntiles = (it.nchunks + 1) / 2;
-      for (int idx = 0; idx < 2 * ntiles; ++idx, ++gidx) {
-        const int j = idx >> 1, kv = idx & 1;
-        // A missing page reads past the pool's end: zeros.
-        const bool have = mine && cur < (uint32_t)a.num_pages;
-        if (kv == 0 && mine && !have && j * kTcPagesPerTile + pj < it.wp.count) {
-          const int32_t at = it.wp.page(j * kTcPagesPerTile + pj);
-          win_report(a.status, kDevErrBadPage, at < it.table ? cur : (uint32_t)at);
-        }
-        const int y = have ? (int)((((int64_t)cur * 2 + kv) * a.Hkv + it.h) * kPageSize) : (int)rows_total;
-        if constexpr (kFp8) {
-          const int su = gidx % kWtStages;
-          ok = __all_sync(0xffffffffu, gidx < kWtStages ||
-                                           mbar_wait(&bars.st_empty[su], ((gidx / kWtStages) - 1) & 1, abort, err));
-          if (!ok) break;
-          const uint32_t present = __ballot_sync(0xffffffffu, have);
-          if (lane == 0)
-            mbar_arrive_expect_tx(&bars.st_full[su],
-                                  Cfg::kCodes + (KV == DD_DTYPE_MXFP8 ? __popc(present) * (Cfg::kExps / 8) : 0));
-          __syncwarp();
-          if (mine) {
-            tma_load_2d(stages + su * Cfg::kCodes + pj * kPageSize * D, &kv_map, 0, y, &bars.st_full[su]);
-            if (KV == DD_DTYPE_MXFP8 && have)
-              bulk_load(stage_exps + su * Cfg::kExps + pj * (Cfg::kExps / 8),
-                        reinterpret_cast<const uint8_t*>(a.scales) + (int64_t)y * (D / 32), Cfg::kExps / 8,
-                        &bars.st_full[su]);
+  } else {
+    if constexpr (kHeld) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::kRegsRest) : "memory");
+    if (warp == Cfg::kProducer) {
+      // ---------------------------------------------------------------- producer
+      const int64_t rows_total = (int64_t)a.num_pages * 2 * a.Hkv * kPageSize;
+      const int pj = lane & (kTcPagesPerTile - 1);
+      const bool mine = lane < kTcPagesPerTile;
+      int gidx = 0;
+      bool ok = true;
+      while (ok && next_item(it)) {
+        uint32_t cur = wt_entry(a, it, pj), nxt = 0xFFFFFFFFu;
+        const int ntiles = (it.nchunks + 1) / 2;
+        for (int idx = 0; idx < 2 * ntiles; ++idx, ++gidx) {
+          const int j = idx >> 1, kv = idx & 1;
+          // A missing page reads past the pool's end: zeros.
+          const bool have = mine && cur < (uint32_t)a.num_pages;
+          if (kv == 0 && mine && !have && j * kTcPagesPerTile + pj < it.wp.count) {
+            const int32_t at = it.wp.page(j * kTcPagesPerTile + pj);
+            win_report(a.status, kDevErrBadPage, at < it.table ? cur : (uint32_t)at);
           }
-        } else {
-          const int s = gidx % kSlots;
-          ok = __all_sync(0xffffffffu, gidx < kSlots ||
-                                           mbar_wait(&bars.kv_empty[s], ((gidx / kSlots) - 1) & 1, abort, err));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&bars.kv_full[s], kTile);
-          __syncwarp();
-          if (mine) {
-            uint8_t* dst = slots + s * kTile + pj * 2048;
-#pragma unroll
-            for (int hf = 0; hf < Cfg::kHalves; ++hf) tma_load_2d(dst + hf * kHalf, &kv_map, 64 * hf, y, &bars.kv_full[s]);
+          const int y = have ? (int)((((int64_t)cur * 2 + kv) * a.Hkv + it.h) * kPageSize) : (int)rows_total;
+          if constexpr (kFp8) {
+            const int su = gidx % kWtStages;
+            ok = __all_sync(0xffffffffu, gidx < kWtStages ||
+                                             mbar_wait(&bars.st_empty[su], ((gidx / kWtStages) - 1) & 1, abort, err));
+            if (!ok) break;
+            const uint32_t present = __ballot_sync(0xffffffffu, have);
+            if (lane == 0)
+              mbar_arrive_expect_tx(&bars.st_full[su],
+                                    Cfg::kCodes + (KV == DD_DTYPE_MXFP8 ? __popc(present) * (Cfg::kExps / 8) : 0));
+            __syncwarp();
+            if (mine) {
+              tma_load_2d(stages + su * Cfg::kCodes + pj * kPageSize * D, &kv_map, 0, y, &bars.st_full[su]);
+              if (KV == DD_DTYPE_MXFP8 && have)
+                bulk_load(stage_exps + su * Cfg::kExps + pj * (Cfg::kExps / 8),
+                          reinterpret_cast<const uint8_t*>(a.scales) + (int64_t)y * (D / 32), Cfg::kExps / 8,
+                          &bars.st_full[su]);
+            }
+          } else {
+            const int s = gidx % kSlots;
+            ok = __all_sync(0xffffffffu, gidx < kSlots ||
+                                             mbar_wait(&bars.kv_empty[s], ((gidx / kSlots) - 1) & 1, abort, err));
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&bars.kv_full[s], kTile);
+            __syncwarp();
+            if (mine) {
+              uint8_t* dst = slots + s * kTile + pj * 2048;
+  #pragma unroll
+              for (int hf = 0; hf < Cfg::kHalves; ++hf) tma_load_2d(dst + hf * kHalf, &kv_map, 64 * hf, y, &bars.kv_full[s]);
+            }
           }
+          if (kv == 0)
+            nxt = wt_entry(a, it, (j + 1) * kTcPagesPerTile + pj);
+          else
+            cur = nxt;
         }
-        if (kv == 0)
-          nxt = wt_entry(a, it, (j + 1) * kTcPagesPerTile + pj);
-        else
-          cur = nxt;
       }
-    }
-  } else if (warp <= Cfg::kProducer + 2) {
-    // ----------------------------------------------------------------- issuers
-    // A warp for each sub-tile: a product is accepted only when the one before
-    // it has all but run, and even a wait for a barrier that is already complete
-    // costs 85 cycles, so one warp for both left the tensor core idle at every
-    // wait. The whole warp walks the list, every branch taken on a vote, and one
-    // elected lane issues, several products to an asm block.
-    const int x = warp - Cfg::kProducer - 1;
-    const uint32_t q_addr = (smem_u32(q_s) + x * kTile) >> 4, s_addr = smem_u32(slots) >> 4;
-    const uint32_t tb = uniform(tbase);
-    int g0 = 0;              // ring index of the item's first K tile
-    int n = 0;               // items of this sub-tile
-    int turns = 0;           // turns taken
-    int used[2] = {0, 0};    // its first and second halves of tiles
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, int phase) {
-      const bool all = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, abort, err));
-      tc_fence_after();
-      return all;
-    };
-    while (ok) {
-      next_item(it);
-      const int nchunks = uniform(it.nchunks), ntok = uniform(it.ntok);
-      if (ntok <= 0) break;
-      const int ntiles = (nchunks + 1) / 2;
-      if (ntok <= x * sub) {
-        // Nothing to issue here: the tiles are given back as they come.
-        for (int i = g0; ok && i < g0 + 2 * ntiles; ++i) {
-          ok = wait(&bars.kv_full[i % kSlots], i / kSlots);
-          if (ok && lane == 0) mbar_arrive(&bars.kv_empty[i % kSlots]);
+    } else if (warp <= Cfg::kProducer + 2) {
+      // ----------------------------------------------------------------- issuers
+      // A warp for each sub-tile: a product is accepted only when the one before
+      // it has all but run, and even a wait for a barrier that is already complete
+      // costs 85 cycles, so one warp for both left the tensor core idle at every
+      // wait. The whole warp walks the list, every branch taken on a vote, and one
+      // elected lane issues, several products to an asm block.
+      const int x = warp - Cfg::kProducer - 1;
+      const uint32_t q_addr = (smem_u32(q_s) + x * kTile) >> 4, s_addr = smem_u32(slots) >> 4;
+      const uint32_t tb = uniform(tbase);
+      int g0 = 0;              // ring index of the item's first K tile
+      int n = 0;               // items of this sub-tile
+      int turns = 0;           // turns taken
+      int used[2] = {0, 0};    // its first and second halves of tiles
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, int phase) {
+        const bool all = __all_sync(0xffffffffu, mbar_wait(bar, phase & 1, abort, err));
+        tc_fence_after();
+        return all;
+      };
+      while (ok) {
+        next_item(it);
+        const int nchunks = uniform(it.nchunks), ntok = uniform(it.ntok);
+        if (ntok <= 0) break;
+        const int ntiles = (nchunks + 1) / 2;
+        if (ntok <= x * sub) {
+          // Nothing to issue here: the tiles are given back as they come.
+          for (int i = g0; ok && i < g0 + 2 * ntiles; ++i) {
+            ok = wait(&bars.kv_full[i % kSlots], i / kSlots);
+            if (ok && lane == 0) mbar_arrive(&bars.kv_empty[i % kSlots]);
+            __syncwarp();
+          }
+          g0 += 2 * ntiles;
+          continue;
+        }
+        if (nchunks == 0) continue;
+        // With both sub-tiles at work their products are issued in turn, a tile's
+        // last P.V and the next Q.K together: issued as they come, both sub-tiles
+        // fall into step, their softmaxes share the exponential unit and then
+        // their products the tensor core (4650 cycles a tile).
+        const bool both = ntok > sub;
+        auto my_turn = [&]() { return !both || wait(&bars.turn[x], turns++); };
+        auto your_turn = [&]() {
+          if (both && lane == 0) mbar_arrive(&bars.turn[1 - x]);
           __syncwarp();
+        };
+        // Scores of tile j; what is free after them.
+        auto issue_qk = [&](int j) {
+          const int slot = (g0 + 2 * j) % kSlots;
+          umma_qk<D, Cfg::kIdQK>(tb + col_s(x), q_addr, s_addr + (slot * kTile >> 4), kHalf >> 4);
+          umma_commit_one(&bars.s_full[x]);
+          umma_commit_one(&bars.kv_empty[slot]);
+          if (j == ntiles - 1) umma_commit_one(&bars.q_empty[x]);
+        };
+        ok = wait(&bars.q_full[x], n++) && wait(&bars.kv_full[g0 % kSlots], g0 / kSlots) && my_turn();
+        if (!ok) break;
+        issue_qk(0);
+        your_turn();
+        for (int j = 0; ok && j < ntiles; ++j) {
+          const int vi = g0 + 2 * j + 1, ki = vi + 1, slot = vi % kSlots;
+          const uint32_t o = tb + col_o(x), p = tb + col_s(x), v = s_addr + (slot * kTile >> 4);
+          const bool two = 2 * j + 1 < nchunks, more = j + 1 < ntiles;
+          ok = wait(&bars.kv_full[slot], vi / kSlots) && (!more || wait(&bars.kv_full[ki % kSlots], ki / kSlots));
+          if (two) {
+            ok = ok && wait(&bars.p_full[x][1], used[1]++);
+            if (!ok) break;
+            umma_pv<Cfg::kIdPV>(o, p + kWtChunk, v + (kWtChunk * 128 >> 4), kHalf >> 4, j > 0 ? 1u : 0u);
+          }
+          ok = ok && my_turn() && wait(&bars.p_full[x][0], used[0]++);
+          if (!ok) break;
+          umma_pv<Cfg::kIdPV>(o, p, v, kHalf >> 4, j > 0 || two ? 1u : 0u);
+          umma_commit_one(&bars.kv_empty[slot]);
+          if (more)
+            issue_qk(j + 1);
+          else
+            umma_commit_one(&bars.o_full[x]);
+          your_turn();
         }
         g0 += 2 * ntiles;
-        continue;
       }
-      if (nchunks == 0) continue;
-      // With both sub-tiles at work their products are issued in turn, a tile's
-      // last P.V and the next Q.K together: issued as they come, both sub-tiles
-      // fall into step, their softmaxes share the exponential unit and then
-      // their products the tensor core (4650 cycles a tile).
-      const bool both = ntok > sub;
-      auto my_turn = [&]() { return !both || wait(&bars.turn[x], turns++); };
-      auto your_turn = [&]() {
-        if (both && lane == 0) mbar_arrive(&bars.turn[1 - x]);
+    } else {
+      // --------------------------------------------------- scheduler and Q loader
+      // Publishes item k + 1 (and asks for its Q in L2), then loads the Q of item
+      // k once the scores of item k - 1 are done.
+      int n[2] = {0, 0};
+      bool ok = true, have = false;
+      const bool tiled = a.gqa_map == DD_GQA_TILED;
+      WtItem nx;
+      it.ntok = 0;
+      for (int i = 0, k = 0;; ++i) {
+        const bool more = wt_item(a, units, 2 * sub, i, nx);
+        if (!more) nx.ntok = -1;
+        if (nx.ntok == 0) continue;
+        const int s = k % kWtItems;
+        ok = __all_sync(0xffffffffu, k < kWtItems || mbar_wait(&bars.item_empty[s], ((k / kWtItems) - 1) & 1, abort, err));
+        if (!ok) break;
+        if (lane == 0) {
+          bars.items[s] = nx;
+          mbar_arrive(&bars.item_full[s]);
+          if (more && nx.nchunks > 0)
+            for (int x = 0; x < 2 && nx.ntok > x * sub; ++x)
+              for (int hf = 0; hf < Cfg::kHalves; ++hf)
+                prefetch_tma_4d(&q_map, 64 * hf, tiled ? nx.h : 0, tiled ? 0 : nx.h, nx.row + x * sub);
+        }
         __syncwarp();
-      };
-      // Scores of tile j; what is free after them.
-      auto issue_qk = [&](int j) {
-        const int slot = (g0 + 2 * j) % kSlots;
-        umma_qk<D, Cfg::kIdQK>(tb + col_s(x), q_addr, s_addr + (slot * kTile >> 4), kHalf >> 4);
-        umma_commit_one(&bars.s_full[x]);
-        umma_commit_one(&bars.kv_empty[slot]);
-        if (j == ntiles - 1) umma_commit_one(&bars.q_empty[x]);
-      };
-      ok = wait(&bars.q_full[x], n++) && wait(&bars.kv_full[g0 % kSlots], g0 / kSlots) && my_turn();
-      if (!ok) break;
-      issue_qk(0);
-      your_turn();
-      for (int j = 0; ok && j < ntiles; ++j) {
-        const int vi = g0 + 2 * j + 1, ki = vi + 1, slot = vi % kSlots;
-        const uint32_t o = tb + col_o(x), p = tb + col_s(x), v = s_addr + (slot * kTile >> 4);
-        const bool two = 2 * j + 1 < nchunks, more = j + 1 < ntiles;
-        ok = wait(&bars.kv_full[slot], vi / kSlots) && (!more || wait(&bars.kv_full[ki % kSlots], ki / kSlots));
-        if (two) {
-          ok = ok && wait(&bars.p_full[x][1], used[1]++);
-          if (!ok) break;
-          umma_pv<Cfg::kIdPV>(o, p + kWtChunk, v + (kWtChunk * 128 >> 4), kHalf >> 4, j > 0 ? 1u : 0u);
-        }
-        ok = ok && my_turn() && wait(&bars.p_full[x][0], used[0]++);
-        if (!ok) break;
-        umma_pv<Cfg::kIdPV>(o, p, v, kHalf >> 4, j > 0 || two ? 1u : 0u);
-        umma_commit_one(&bars.kv_empty[slot]);
-        if (more)
-          issue_qk(j + 1);
-        else
-          umma_commit_one(&bars.o_full[x]);
-        your_turn();
-      }
-      g0 += 2 * ntiles;
-    }
-  } else {
-    // --------------------------------------------------- scheduler and Q loader
-    // Publishes item k + 1 (and asks for its Q in L2), then loads the Q of item
-    // k once the scores of item k - 1 are done.
-    int n[2] = {0, 0};
-    bool ok = true, have = false;
-    const bool tiled = a.gqa_map == DD_GQA_TILED;
-    WtItem nx;
-    it.ntok = 0;
-    for (int i = 0, k = 0;; ++i) {
-      const bool more = wt_item(a, units, 2 * sub, i, nx);
-      if (!more) nx.ntok = -1;
-      if (nx.ntok == 0) continue;
-      const int s = k % kWtItems;
-      ok = __all_sync(0xffffffffu, k < kWtItems || mbar_wait(&bars.item_empty[s], ((k / kWtItems) - 1) & 1, abort, err));
-      if (!ok) break;
-      if (lane == 0) {
-        bars.items[s] = nx;
-        mbar_arrive(&bars.item_full[s]);
-        if (more && nx.nchunks > 0)
-          for (int x = 0; x < 2 && nx.ntok > x * sub; ++x)
-            for (int hf = 0; hf < Cfg::kHalves; ++hf)
-              prefetch_tma_4d(&q_map, 64 * hf, tiled ? nx.h : 0, tiled ? 0 : nx.h, nx.row + x * sub);
-      }
-      __syncwarp();
-      ++k;
-      if (have) {
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if (it.nchunks == 0 || it.ntok <= x * sub) break;
-          ok = __all_sync(0xffffffffu, n[x] == 0 || mbar_wait(&bars.q_empty[x], (n[x] - 1) & 1, abort, err));
-          if (!ok) break;
-          ++n[x];
-          if (lane == 0) {
-            uint64_t* bar = kF16 ? &bars.q_raw[x] : &bars.q_full[x];
-            mbar_arrive_expect_tx(bar, Cfg::kHalves * sub * a.g * 128);
-#pragma unroll
-            for (int hf = 0; hf < Cfg::kHalves; ++hf)
-              tma_load_4d(q_s + x * kTile + hf * kHalf, &q_map, 64 * hf, tiled ? it.h : 0, tiled ? 0 : it.h,
-                          it.row + x * sub, bar);
+        ++k;
+        if (have) {
+  #pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (it.nchunks == 0 || it.ntok <= x * sub) break;
+            ok = __all_sync(0xffffffffu, n[x] == 0 || mbar_wait(&bars.q_empty[x], (n[x] - 1) & 1, abort, err));
+            if (!ok) break;
+            ++n[x];
+            if (lane == 0) {
+              uint64_t* bar = kF16 ? &bars.q_raw[x] : &bars.q_full[x];
+              mbar_arrive_expect_tx(bar, Cfg::kHalves * sub * a.g * 128);
+  #pragma unroll
+              for (int hf = 0; hf < Cfg::kHalves; ++hf)
+                tma_load_4d(q_s + x * kTile + hf * kHalf, &q_map, 64 * hf, tiled ? it.h : 0, tiled ? 0 : it.h,
+                            it.row + x * sub, bar);
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          if (!ok) break;
         }
-        if (!ok) break;
+        if (!more) break;
+        it = nx;
+        have = true;
       }
-      if (!more) break;
-      it = nx;
-      have = true;
     }
   }
   tc_fence_before();
@@ -802,6 +827,14 @@ static cudaError_t launch_win_tc_t(const CUtensorMap& kv, const CUtensorMap& q, 
   using Cfg = WtCfg<D, KV>;
   cudaError_t e = cudaFuncSetAttribute(win_tc_kernel<D, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
   if (e != cudaSuccess) return e;
+  if (Cfg::kHeld) {
+    // setmaxnreg.inc waits for registers that the block does not have if it
+    // was launched with fewer.
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, win_tc_kernel<D, KV>);
+    if (e != cudaSuccess) return e;
+    if (fa.numRegs < Cfg::kRegs) return cudaErrorInvalidConfiguration;
+  }
   ProfScope ps(kProfTc, st);
   win_tc_kernel<D, KV><<<std::min(units, sms), Cfg::kThreads, Cfg::kSmem, st>>>(kv, q, a, units);
   return cudaGetLastError();
