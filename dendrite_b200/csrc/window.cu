@@ -138,11 +138,11 @@ int launch_win_simple(const WinArgs& a, cudaStream_t st) {
 // Chunks: which of the two tensor-core kernels. Both walk the visible pages of
 // every KV head, the streaming kernel once for 16 rows at about 1.5 ns a page
 // for the whole GPU (two pages' bytes from L2, or HBM), the tcgen05 kernel once
-// for up to 256 rows at 2.4 / 2.7 / 3.2 us (bf16 / E4M3 / MXFP8) for 8 pages on
+// for up to 256 rows at 1.9 / 1.9 / 2.15 us (bf16 / E4M3 / MXFP8) for 8 pages on
 // one SM. Measured around the border (streaming, tcgen05; us), windows of 1024,
-// 2048, 4096 tokens: 64 sequences x 4 new tokens, bf16, 4 heads a group 63, 82;
-// x 8 110, 82; E4M3, 8 heads a group x 4 168, 162; x 8 287, 200; MXFP8 x 8 349,
-// 373; x 16 603, 466; one sequence x 32 MXFP8 28, 94; 4 x 32 E4M3 69, 48.
+// 2048, 4096 tokens: 64 sequences x 4 new tokens, bf16, 4 heads a group 63, 79;
+// x 8 110, 79; E4M3, 8 heads a group x 2 91, 138; x 4 167, 138; MXFP8, 4 heads a
+// group x 4 188, 287; x 8 349, 288; one sequence x 32 27, 75; 4 x 32 E4M3 68, 46.
 static bool tc_is_faster(const WinArgs& a, int max_pages) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
@@ -151,7 +151,7 @@ static bool tc_is_faster(const WinArgs& a, int max_pages) {
   if (a.window > 0) pages = std::min(pages, ((int64_t)a.window + a.sinks + tokens) / kPageSize + 2);
   const int64_t tiles16 = std::max<int64_t>(a.num_seqs, (rows + 15) / 16) * a.Hkv;
   const int64_t items = std::max<int64_t>(a.num_seqs, (rows + 255) / 256) * a.Hkv;
-  const int64_t tile_ns = a.kv_dtype == DD_DTYPE_BF16 ? 2400 : a.kv_dtype == DD_DTYPE_E4M3 ? 2700 : 3200;
+  const int64_t tile_ns = a.kv_dtype == DD_DTYPE_MXFP8 ? 2150 : 1900;
   const int64_t stream_ns = 7000 + tiles16 * pages * 3 / 2;
   const int64_t tc_ns = (items + sms - 1) / sms * (pages * tile_ns / 8 + 4000);
   return tc_ns < stream_ns;

@@ -6,9 +6,12 @@
 // sub-tile's rows being (token, query head of the group): up to 128 rows of Q,
 // which one TMA box brings. The item's pages are those that its first token's
 // window up to its last token's position reach, plus those of the first tokens.
-// Persistent CTAs, one per SM, take the items in a fixed order, long ones (late
-// tokens) first, the direction of every second round reversed; nothing is
-// planned on the host. K and V come in tiles of 128 tokens (8 pages of the
+// The launch has a CTA per item, long ones (late tokens) first. Each CTA that
+// has started (one per SM) claims further ones in place of their starting, as
+// it comes near the end of its item; nothing is planned on the host. (A fixed
+// share of the items for each CTA took 908 us in place of 799 for 16 chunks of
+// 200 to 2000 tokens, bf16, window 4096, and 291 in place of 270 for 4 chunks of
+// 1000, E4M3, window 2048.) K and V come in tiles of 128 tokens (8 pages of the
 // item's list):
 //   softmax      warps 0-3 sub-tile A, 4-7 B, a thread per row: the maximum of
 //                128 scores in TMEM, then the weights of the tile's second and
@@ -18,7 +21,7 @@
 //   producer     TMA boxes of K and V into the ring (FP8 codes: into a staging
 //                ring); lane p < 8 looks page p of a tile up
 //   issuers      one per sub-tile: per tile P.V by halves, then the next Q.K
-//   scheduler    the items, one ahead, into a small ring that the others read
+//   scheduler    claims the items, into a small ring that the others read
 //                (finding an item is a chain of dependent loads and divisions),
 //                and an item's Q once the previous item's last scores are done
 // The tensor core works on one sub-tile while the softmax of the other runs.
@@ -94,6 +97,7 @@ struct WtItem {
 };
 
 constexpr int kWtItems = 2;  // items of the ring
+constexpr int kWtAhead = 2;  // tiles of an item still to be asked for when the next is claimed
 struct WtBars {
   uint64_t kv_full[4], kv_empty[4];
   uint64_t st_full[kWtStages], st_empty[kWtStages];
@@ -104,27 +108,27 @@ struct WtBars {
   uint64_t q_raw[2];                    // f16: bf16 rows of Q in place, to be converted
   uint64_t q_full[2], q_empty[2];       // Q ready / the item's last scores done
   uint64_t item_full[kWtItems], item_empty[kWtItems];
+  uint64_t late;                        // an item's last tiles are being asked for
+  uint64_t claim;                       // the answer to a claim has come
   WtItem items[kWtItems];
+  alignas(16) uint4 answer;
   uint32_t tmem_base;
   int abort;
 };
 
-// Item `i` of this CTA; false past the end. Tiles are counted in tokens: `per`
-// of them make an item. The launch keeps units and rows * g below 2^31.
-__device__ __forceinline__ bool wt_item(const WinArgs& a, int32_t units, int32_t per, int32_t i, WtItem& it) {
-  const int32_t n = (int32_t)gridDim.x, first = i * n;
-  if (first >= units) return false;
-  const int32_t u = first + ((i & 1) ? n - 1 - (int32_t)blockIdx.x : (int32_t)blockIdx.x);
+// Unit `u` of the launch, late tokens first; ntok = 0 for a surplus one. Tiles
+// are counted in tokens: `per` of them make an item. The launch keeps units and
+// rows * g below 2^31.
+__device__ __forceinline__ void wt_item(const WinArgs& a, int32_t per, int32_t u, WtItem& it) {
+  const uint32_t unit = gridDim.x - 1 - (uint32_t)u, tile_id = unit / (uint32_t)a.Hkv;
   it.ntok = 0;
-  if (u >= units) return true;
-  const uint32_t unit = (uint32_t)(units - 1 - u), tile_id = unit / (uint32_t)a.Hkv;
   it.h = (int32_t)(unit - tile_id * (uint32_t)a.Hkv);
   int32_t s, tile;
   win_tile(a, 1, per, tile_id, s, tile);
   const SeqRows sr = seq_rows(a.row_indptr, a.num_tokens, a.num_rows, s);
-  if (tile < 0 || tile > sr.m / per) return true;
+  if (tile < 0 || tile > sr.m / per) return;
   it.ntok = min(per, sr.m - tile * per);
-  if (it.ntok <= 0) return true;
+  if (it.ntok <= 0) return;
   it.row = sr.r0 + tile * per;
   it.p_lo = sr.pos0 + tile * per;
   it.p_hi = it.p_lo + it.ntok - 1;
@@ -133,7 +137,6 @@ __device__ __forceinline__ bool wt_item(const WinArgs& a, int32_t units, int32_t
   it.wp = win_pages(a.window, a.sinks, it.p_lo, it.p_hi);
   it.shift = (it.wp.wp - it.wp.ns) * kPageSize;
   it.nchunks = (it.wp.count + kWtChunk / kPageSize - 1) / (kWtChunk / kPageSize);
-  return true;
 }
 // Table entry of page v of the item's list as it stands (0xFFFFFFFF past the
 // list or the table): looked up a tile ahead, and judged when it is used, so
@@ -211,6 +214,25 @@ __device__ __forceinline__ void umma_pv(uint32_t d, uint32_t p, uint32_t b, uint
       " @l tcgen05.mma.cta_group::1.kind::f16 [%0], [p], db, %4, t;\n}" ::"r"(d),
       "r"(p), "r"(b), "n"(kWtDescHi), "n"(kId), "r"(acc));
 }
+// Claims a CTA of this launch that has not started yet (16 bytes at `answer`,
+// counted by `bar`), and its index; -1 if there is none left.
+__device__ __forceinline__ void claim_cta(uint4* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ int32_t claimed_cta(const uint4* answer) {
+  int32_t u;
+  asm volatile(
+      "{\n .reg .b128 r;\n .reg .pred p;\n ld.shared.b128 r, [%1];\n mov.b32 %0, -1;\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n}"
+      : "=r"(u)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return u;
+}
 // 4-D TMA load (Q rows: dims, heads, head groups, tokens).
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z,
                                             int32_t w, uint64_t* bar) {
@@ -276,8 +298,7 @@ __device__ __forceinline__ void wt_weights(const float (&s)[32], uint64_t sc2, u
 
 template <int D, int KV>
 __global__ void __maxnreg__((WtCfg<D, KV>::kRegs))
-    win_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, WinArgs a,
-                  int32_t units) {
+    win_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, WinArgs a) {
   using Cfg = WtCfg<D, KV>;
   constexpr bool kFp8 = Cfg::kFp8, kF16 = Cfg::kF16, kHeld = Cfg::kHeld;
   constexpr int kSlots = Cfg::kSlots, kTile = Cfg::kTileBytes, kHalf = Cfg::kHalfBytes;
@@ -314,6 +335,8 @@ __global__ void __maxnreg__((WtCfg<D, KV>::kRegs))
       mbar_init(&bars.item_full[s], 1);
       mbar_init(&bars.item_empty[s], 8 + (kFp8 ? kWtConvWarps : 0) + 3);
     }
+    mbar_init(&bars.late, 1);
+    mbar_init(&bars.claim, 1);
     bars.abort = 0;
     fence_mbar_init();
     mbar_arrive(&bars.turn[0]);  // sub-tile A begins
@@ -648,9 +671,11 @@ __global__ void __maxnreg__((WtCfg<D, KV>::kRegs))
       bool ok = true;
       while (ok && next_item(it)) {
         uint32_t cur = wt_entry(a, it, pj), nxt = 0xFFFFFFFFu;
-        const int ntiles = (it.nchunks + 1) / 2;
+        const int ntiles = (it.nchunks + 1) / 2, late = 2 * max(ntiles - kWtAhead, 0);
+        if (ntiles == 0 && lane == 0) mbar_arrive(&bars.late);
         for (int idx = 0; idx < 2 * ntiles; ++idx, ++gidx) {
           const int j = idx >> 1, kv = idx & 1;
+          if (idx == late && lane == 0) mbar_arrive(&bars.late);
           // A missing page reads past the pool's end: zeros.
           const bool have = mine && cur < (uint32_t)a.num_pages;
           if (kv == 0 && mine && !have && j * kTcPagesPerTile + pj < it.wp.count) {
@@ -776,57 +801,75 @@ __global__ void __maxnreg__((WtCfg<D, KV>::kRegs))
       }
     } else {
       // --------------------------------------------------- scheduler and Q loader
-      // Publishes item k + 1 (and asks for its Q in L2), then loads the Q of item
-      // k once the scores of item k - 1 are done.
-      int n[2] = {0, 0};
-      bool ok = true, have = false;
+      // Publishes an item, loads its Q once the scores of the one before are
+      // done, and claims the next when the item's last tiles are asked for.
+      int n[2] = {0, 0}, claims = 0;
+      int32_t u = (int32_t)blockIdx.x;
+      bool ok = true;
       const bool tiled = a.gqa_map == DD_GQA_TILED;
-      WtItem nx;
-      it.ntok = 0;
-      for (int i = 0, k = 0;; ++i) {
-        const bool more = wt_item(a, units, 2 * sub, i, nx);
-        if (!more) nx.ntok = -1;
-        if (nx.ntok == 0) continue;
+      auto claim = [&]() {
+        __syncwarp();
+        if (lane == 0) {
+          fence_proxy_async_smem();  // the last answer has been read
+          mbar_arrive_expect_tx(&bars.claim, 16);
+          claim_cta(&bars.answer, &bars.claim);
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars.claim, claims++ & 1, abort, err));
+        u = ok && lane == 0 ? claimed_cta(&bars.answer) : -1;
+        u = __shfl_sync(0xffffffffu, u, 0);
+      };
+      for (int k = 0;; ++k) {
+        it.ntok = -1;
+        while (u >= 0) {
+          wt_item(a, 2 * sub, u, it);
+          if (it.ntok > 0) break;
+          it.ntok = -1;
+          claim();
+        }
         const int s = k % kWtItems;
-        ok = __all_sync(0xffffffffu, k < kWtItems || mbar_wait(&bars.item_empty[s], ((k / kWtItems) - 1) & 1, abort, err));
+        ok = ok && __all_sync(0xffffffffu, k < kWtItems || mbar_wait(&bars.item_empty[s], ((k / kWtItems) - 1) & 1, abort, err));
         if (!ok) break;
         if (lane == 0) {
-          bars.items[s] = nx;
+          bars.items[s] = it;
           mbar_arrive(&bars.item_full[s]);
-          if (more && nx.nchunks > 0)
-            for (int x = 0; x < 2 && nx.ntok > x * sub; ++x)
-              for (int hf = 0; hf < Cfg::kHalves; ++hf)
-                prefetch_tma_4d(&q_map, 64 * hf, tiled ? nx.h : 0, tiled ? 0 : nx.h, nx.row + x * sub);
         }
         __syncwarp();
-        ++k;
-        if (have) {
-  #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (it.nchunks == 0 || it.ntok <= x * sub) break;
-            ok = __all_sync(0xffffffffu, n[x] == 0 || mbar_wait(&bars.q_empty[x], (n[x] - 1) & 1, abort, err));
-            if (!ok) break;
-            ++n[x];
-            if (lane == 0) {
-              uint64_t* bar = kF16 ? &bars.q_raw[x] : &bars.q_full[x];
-              mbar_arrive_expect_tx(bar, Cfg::kHalves * sub * a.g * 128);
-  #pragma unroll
-              for (int hf = 0; hf < Cfg::kHalves; ++hf)
-                tma_load_4d(q_s + x * kTile + hf * kHalf, &q_map, 64 * hf, tiled ? it.h : 0, tiled ? 0 : it.h,
-                            it.row + x * sub, bar);
-            }
-            __syncwarp();
-          }
+        if (u < 0) break;
+        // Into L2 first, while the buffers are still in use.
+        if (lane == 0 && it.nchunks > 0)
+          for (int x = 0; x < 2 && it.ntok > x * sub; ++x)
+            for (int hf = 0; hf < Cfg::kHalves; ++hf)
+              prefetch_tma_4d(&q_map, 64 * hf, tiled ? it.h : 0, tiled ? 0 : it.h, it.row + x * sub);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if (it.nchunks == 0 || it.ntok <= x * sub) break;
+          ok = __all_sync(0xffffffffu, n[x] == 0 || mbar_wait(&bars.q_empty[x], (n[x] - 1) & 1, abort, err));
           if (!ok) break;
+          ++n[x];
+          if (lane == 0) {
+            uint64_t* bar = kF16 ? &bars.q_raw[x] : &bars.q_full[x];
+            mbar_arrive_expect_tx(bar, Cfg::kHalves * sub * a.g * 128);
+#pragma unroll
+            for (int hf = 0; hf < Cfg::kHalves; ++hf)
+              tma_load_4d(q_s + x * kTile + hf * kHalf, &q_map, 64 * hf, tiled ? it.h : 0, tiled ? 0 : it.h,
+                          it.row + x * sub, bar);
+          }
+          __syncwarp();
         }
-        if (!more) break;
-        it = nx;
-        have = true;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&bars.late, k & 1, abort, err));
+        if (!ok) break;
+        claim();
+        if (!ok) break;
       }
     }
   }
   tc_fence_before();
   __syncthreads();
+  if (*abort) {  // a wait ran out: what is still in flight lands before the CTA leaves
+    const uint64_t t0 = global_ns();
+    while (global_ns() - t0 < 200000) {
+    }
+  }
   if (warp == Cfg::kProducer + 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "r"(kTmemCols)
@@ -841,7 +884,7 @@ int make_q_tensor_map(CUtensorMap* map, const void* q, int64_t rows, int64_t row
 
 template <int D, int KV>
 static cudaError_t launch_win_tc_t(const CUtensorMap& kv, const CUtensorMap& q, const WinArgs& a, int32_t units,
-                                   int sms, cudaStream_t st) {
+                                   cudaStream_t st) {
   using Cfg = WtCfg<D, KV>;
   cudaError_t e = cudaFuncSetAttribute(win_tc_kernel<D, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
   if (e != cudaSuccess) return e;
@@ -854,16 +897,16 @@ static cudaError_t launch_win_tc_t(const CUtensorMap& kv, const CUtensorMap& q, 
     if (fa.numRegs < Cfg::kRegs) return cudaErrorInvalidConfiguration;
   }
   ProfScope ps(kProfTc, st);
-  win_tc_kernel<D, KV><<<std::min(units, sms), Cfg::kThreads, Cfg::kSmem, st>>>(kv, q, a, units);
+  win_tc_kernel<D, KV><<<units, Cfg::kThreads, Cfg::kSmem, st>>>(kv, q, a);
   return cudaGetLastError();
 }
 template <int D>
 static cudaError_t launch_win_tc_kv(const CUtensorMap& kv, const CUtensorMap& q, const WinArgs& a, int32_t units,
-                                    int sms, cudaStream_t st) {
+                                    cudaStream_t st) {
   switch (a.kv_dtype) {
-    case DD_DTYPE_BF16: return launch_win_tc_t<D, DD_DTYPE_BF16>(kv, q, a, units, sms, st);
-    case DD_DTYPE_E4M3: return launch_win_tc_t<D, DD_DTYPE_E4M3>(kv, q, a, units, sms, st);
-    default: return launch_win_tc_t<D, DD_DTYPE_MXFP8>(kv, q, a, units, sms, st);
+    case DD_DTYPE_BF16: return launch_win_tc_t<D, DD_DTYPE_BF16>(kv, q, a, units, st);
+    case DD_DTYPE_E4M3: return launch_win_tc_t<D, DD_DTYPE_E4M3>(kv, q, a, units, st);
+    default: return launch_win_tc_t<D, DD_DTYPE_MXFP8>(kv, q, a, units, st);
   }
 }
 
@@ -880,15 +923,13 @@ bool win_tc_fits(const WinArgs& a) {
 }
 
 int launch_win_tc(const WinArgs& a, cudaStream_t st) {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   CUtensorMap kv, q;
   int rc = make_kv_tensor_map(&kv, a.kv, a.num_pages, a.Hkv, a.D, a.kv_dtype == DD_DTYPE_BF16 ? 2 : 1, 0);
   if (!rc) rc = make_q_tensor_map(&q, a.q, a.num_rows, a.q_stride, a.Hq, a.Hkv, a.D, a.gqa_map, 128 / a.g);
   if (rc) return rc;
   const int32_t units = (int32_t)win_tc_units(a);
-  const cudaError_t e = a.D == 64 ? launch_win_tc_kv<64>(kv, q, a, units, sms, st)
-                                  : launch_win_tc_kv<128>(kv, q, a, units, sms, st);
+  const cudaError_t e = a.D == 64 ? launch_win_tc_kv<64>(kv, q, a, units, st)
+                                  : launch_win_tc_kv<128>(kv, q, a, units, st);
   if (e != cudaSuccess) return fail(DD_ERR_CUDA, std::string("window attention launch: ") + cudaGetErrorString(e));
   return DD_OK;
 }
