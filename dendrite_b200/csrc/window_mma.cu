@@ -660,10 +660,15 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
 // more than whole waves and have pages enough, they are split to even the last
 // one out. (4096-token windows, bf16: 64 sequences of 8 heads, 512 units for
 // 444 places: 220 us whole, 187 in two, 177 in four; 4 sequences: 67 us whole,
-// 17 in eight, 28 in sixteen, which is more than one wave.)
+// 17 in eight.) Sixteen CTAs have to fit one group of SMs, so such clusters
+// fill some 0.6 of the places in one wave, and joining them costs a microsecond
+// that few pages do not repay (a decode step of 1 / 2 / 3 sequences of 8 heads,
+// bf16, 8192-token windows, eight and sixteen: 17.9, 14.8; 21.8, 20.3; 25.6,
+// 35.4 us; 1024-token windows 8.2, 8.7; 8.8, 10.1; 9.1, 17.4).
 static int win_split(int64_t units, int64_t places, int64_t pages) {
   int n = 1;
-  while (n < 16 && units * n * 2 <= places && pages >= 2 * n * kWinWarps) n *= 2;
+  while (n < 8 && units * n * 2 <= places && pages >= 2 * n * kWinWarps) n *= 2;
+  if (n == 8 && units * 16 * 5 <= places * 3 && pages >= 128) n = 16;
   auto last_wave_idle = [&]() {
     const int64_t waves = (units * n + places - 1) / places;
     return units * n * 100 < waves * places * 85;
