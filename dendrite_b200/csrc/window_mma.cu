@@ -3,18 +3,22 @@
 //
 // Few rows read many tokens, so HBM bounds it: the kernel's work is to keep
 // loads in flight and to spend few instructions on each byte.
-//  - A warp takes one 16-token page at a time, straight from global memory
-//    into the fragment registers of its products: no shared memory, no
-//    barriers, every 32-byte sector read whole by one instruction. The
-//    products are transposed, S^T = K Q^T and O^T = V^T P^T (m16n8k16), so
+//  - A warp takes one 16-token page at a time and waits for no other warp. bf16
+//    pages go straight from global memory into the fragment registers of its
+//    products, every 32-byte sector read whole by one instruction. FP8 pages
+//    hold half as many bytes for as many instructions, so registers keep too
+//    little in flight: they come through a ring in shared memory, three pages or
+//    more for each warp (128 x 2048 tokens of E4M3: 89 us, 5.5 TB/s, against 103
+//    through the registers).
+//  - The products are transposed, S^T = K Q^T and O^T = V^T P^T (m16n8k16), so
 //    the page's tokens (and V's head dims) are the 16-row side and the 8-column
 //    side holds NT x 8 query rows: a GQA group of up to 8 wastes no second half.
 //    The head dims of K are contracted in an order in which a lane's share of
 //    a token is contiguous (Q is loaded in the same order); V's dims are dealt
 //    to the product's rows the same way, two tokens' words being interleaved
 //    with byte permutes.
-//  - K of the next page is requested as soon as S is formed, V of the next as
-//    soon as O is: half to all of a page is in flight for every warp.
+//  - bf16: K of the next page is requested as soon as S is formed, V of the next
+//    as soon as O is: half to all of a page is in flight for every warp.
 //  - S^T and O^T have their query row in the same lane, so the softmax state
 //    (reference, sum) and a rescale need no exchange; the reference moves only
 //    when a score passes it by 8 (log2 units), found by one vote a page.
@@ -45,16 +49,6 @@ __device__ __forceinline__ uint4 ldg128(const void* p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ldg64(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint32_t ldg32(const void* p) {
-  uint32_t v;
-  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
   return v;
 }
 __device__ __forceinline__ uint32_t movm_trans(uint32_t a) {
@@ -95,62 +89,96 @@ struct WinFrag {
   uint32_t ek[2][(D + 127) / 128], ev[2][(D + 127) / 128];
 };
 
+// ---- bf16: straight from global memory.
 template <int D>
-__device__ __forceinline__ void load_exps(const uint8_t* p, uint32_t (&e)[(D + 127) / 128]) {
-  if (D == 64) {
-    uint16_t x;
-    asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(x) : "l"(p));
-    e[0] = x;
-  } else if (D == 128) {
-    e[0] = ldg32(p);
-  } else {
-    const uint2 x = ldg64(p);
-    e[0] = x.x;
-    e[(D + 127) / 128 - 1] = x.y;
-  }
-}
-
-template <int D, int KV>
-__device__ __forceinline__ void load_k(WinFrag<D, KV>& f, const WinArgs& a, uint32_t page, int h, int g, int c) {
-  constexpr int kElem = KV == kWinBf16 ? 2 : 1;
+__device__ __forceinline__ void load_k(WinFrag<D, kWinBf16>& f, const WinArgs& a, uint32_t page, int h, int g, int c) {
   const int64_t row = ((int64_t)page * 2 * a.Hkv + h) * kPageSize + g;
-  const uint8_t* p = reinterpret_cast<const uint8_t*>(a.kv) + (row * D + 8 * c) * kElem;
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(a.kv) + row * D + 8 * c;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const uint8_t* q = p + (half * 8 * D + 32 * i) * kElem;
-      if constexpr (KV == kWinBf16)
-        f.k[i][half] = ldg128(q);
-      else
-        f.k[i][half] = ldg64(q);
-    }
-  if constexpr (KV == kWinMx) {
-    const uint8_t* e = reinterpret_cast<const uint8_t*>(a.scales) + row * (D / 32);
-    load_exps<D>(e, f.ek[0]);
-    load_exps<D>(e + 8 * (D / 32), f.ek[1]);
-  }
+    for (int half = 0; half < 2; ++half) f.k[i][half] = ldg128(p + half * 8 * D + 32 * i);
 }
-template <int D, int KV>
-__device__ __forceinline__ void load_v(WinFrag<D, KV>& f, const WinArgs& a, uint32_t page, int h, int g, int c) {
+template <int D>
+__device__ __forceinline__ void load_v(WinFrag<D, kWinBf16>& f, const WinArgs& a, uint32_t page, int h, int g, int c) {
   const int64_t slice = (((int64_t)page * 2 + 1) * a.Hkv + h) * kPageSize;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int64_t row = slice + 2 * c + (j & 1) + 8 * (j >> 1);
-    if constexpr (KV == kWinBf16) {
-      const uint16_t* p = reinterpret_cast<const uint16_t*>(a.kv) + row * D + 8 * g;
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(a.kv) + row * D + 8 * g;
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) f.v[i][j] = ldg128(p + 64 * i);
-    } else {
-      const uint8_t* p = reinterpret_cast<const uint8_t*>(a.kv) + row * D + 4 * g;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) f.v[i][j] = ldg32(p + 32 * i);
-    }
+    for (int i = 0; i < D / 64; ++i) f.v[i][j] = ldg128(p + 64 * i);
   }
+}
+// ---- FP8: a warp's pages come through a ring in shared memory of its own.
+// A slice (16 tokens of K or V of a head) lies there in units of 32 bytes, placed
+// so that the words of eight dims of tokens t .. t + 3 (t = 0, 4; K) and of
+// tokens t, t + 2, t + 4, t + 6 (V) fall into different banks.
+template <int D>
+__device__ __forceinline__ int ring_unit(int t, int b) {
+  if (D == 64) return (t ^ ((t >> 2) & 1)) * 2 + (b ^ ((t >> 1) & 1));
+  return t * (D / 32) + (b ^ ((t >> 1) & 3) ^ ((t & 1) << 1));
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Asks for a page: K, V, then MXFP8's exponents of both.
+template <int D, int KV>
+__device__ __forceinline__ void ring_load(uint32_t stage, const WinArgs& a, uint32_t page, int h, int lane) {
+  const int64_t krow = ((int64_t)page * 2 * a.Hkv + h) * kPageSize, vrow = krow + (int64_t)a.Hkv * kPageSize;
+  const uint8_t* kv = reinterpret_cast<const uint8_t*>(a.kv);
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const int q = lane + 32 * i, t = q / (D / 16), cc = q % (D / 16);
+    const uint32_t dst = stage + ring_unit<D>(t, cc >> 1) * 32 + (cc & 1) * 16;
+    cp_async16(dst, kv + krow * D + q * 16);
+    cp_async16(dst + kPageSize * D, kv + vrow * D + q * 16);
+  }
+  if (KV == kWinMx && lane < 2 * (D / 32)) {
+    const int q = lane % (D / 32);
+    cp_async16(stage + 2 * kPageSize * D + lane * 16,
+               reinterpret_cast<const uint8_t*>(a.scales) + (lane < D / 32 ? krow : vrow) * (D / 32) + q * 16);
+  }
+}
+template <int D>
+__device__ __forceinline__ void ring_exps(const uint8_t* p, uint32_t (&e)[(D + 127) / 128]) {
+  if (D == 64) {
+    e[0] = *reinterpret_cast<const uint16_t*>(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < (D + 127) / 128; ++i) e[i] = reinterpret_cast<const uint32_t*>(p)[i];
+  }
+}
+template <int D, int KV>
+__device__ __forceinline__ void ring_k(WinFrag<D, KV>& f, const uint8_t* stage, int g, int c) {
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      f.k[i][half] = *reinterpret_cast<const uint2*>(stage + ring_unit<D>(g + 8 * half, i) * 32 + 8 * c);
   if constexpr (KV == kWinMx) {
-    const uint8_t* e = reinterpret_cast<const uint8_t*>(a.scales) + (slice + g) * (D / 32);
-    load_exps<D>(e, f.ev[0]);
-    load_exps<D>(e + 8 * (D / 32), f.ev[1]);
+    const uint8_t* e = stage + 2 * kPageSize * D;
+    ring_exps<D>(e + g * (D / 32), f.ek[0]);
+    ring_exps<D>(e + (g + 8) * (D / 32), f.ek[1]);
+  }
+}
+template <int D, int KV>
+__device__ __forceinline__ void ring_v(WinFrag<D, KV>& f, const uint8_t* stage, int g, int c) {
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      f.v[i][j] = *reinterpret_cast<const uint32_t*>(stage + kPageSize * D +
+                                                     ring_unit<D>(2 * c + (j & 1) + 8 * (j >> 1), i) * 32 + 4 * g);
+  if constexpr (KV == kWinMx) {
+    const uint8_t* e = stage + 2 * kPageSize * D + kPageSize * (D / 32);
+    ring_exps<D>(e + g * (D / 32), f.ev[0]);
+    ring_exps<D>(e + (g + 8) * (D / 32), f.ev[1]);
   }
 }
 // Byte b of a word of E8M0 exponents as a power of two (0: 0 in place of
@@ -195,18 +223,31 @@ __device__ __forceinline__ void cluster_barrier() {
 }
 
 // CTAs that an SM holds, as far as the registers go. FP8 pages are half the
-// bytes of bf16 ones and need the fourth (128 x 2048 tokens of E4M3: 102 us; a
-// second page in flight for each warp of three CTAs 126, five CTAs with spills
-// 140).
+// bytes of bf16 ones and need the fourth (128 x 2048 tokens of E4M3: 89 us, in
+// three 97).
 template <int D, int KV, int NT>
 constexpr int kWinCtas = D * NT >= 256 ? 2 : KV == kWinBf16 && D == 128 ? 3 : 4;
+
+// FP8: bytes of a page in the ring, and the pages that a warp's share of the
+// SM's shared memory holds.
+template <int D, int KV, int NT>
+struct WinRing {
+  static constexpr bool kUsed = KV != kWinBf16;
+  static constexpr int kPage = 2 * kPageSize * D + (KV == kWinMx ? 2 * kPageSize * (D / 32) : 0);
+  static constexpr int kPages = kUsed ? (208 * 1024 / kWinCtas<D, KV, NT> / kWinWarps) / kPage : 0;
+  static constexpr int kRing = kWinWarps * kPages * kPage, kState = sizeof(WinShared<D, NT>);
+  static constexpr int kSmem = kRing > kState ? kRing : kState;
+};
 
 template <int D, int KV, int NT>
 __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_kernel(WinArgs a, int nsplit) {
   constexpr int R = NT * 8;
   constexpr bool kF16 = KV != kWinBf16;
   constexpr int kBlocks = D / 32;
-  __shared__ __align__(16) WinShared<D, NT> sh;
+  using Ring = WinRing<D, KV, NT>;
+  constexpr bool kRing = Ring::kUsed;
+  extern __shared__ __align__(16) uint8_t win_smem[];
+  WinShared<D, NT>& sh = *reinterpret_cast<WinShared<D, NT>*>(win_smem);  // once the ring is done
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int rank = blockIdx.x % nsplit;
   const int64_t unit = blockIdx.x / nsplit;
@@ -254,10 +295,30 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
     return __shfl_sync(0xffffffffu, ids, at++);
   };
   WinFrag<D, KV> f;
-  uint32_t now = take(v0 + warp);
-  if (now != 0xFFFFFFFFu) {
-    load_k<D, KV>(f, a, now, h, g, c);
-    load_v<D, KV>(f, a, now, h, g, c);
+  uint32_t now = 0xFFFFFFFFu;
+  uint8_t* ring = win_smem + warp * Ring::kPages * Ring::kPage;
+  int32_t ahead = v0 + warp;  // FP8: the next page to be asked for
+  int ask = 0, slot = 0;      // the ring's places for it and for the current one
+  uint32_t there = 0;         // places that hold a page
+  auto ask_next = [&]() {
+    const uint32_t id = take(ahead);
+    ahead += kWinWarps;
+    there &= ~(1u << ask);
+    if (id != 0xFFFFFFFFu) {
+      ring_load<D, KV>(smem_u32(ring) + ask * Ring::kPage, a, id, h, lane);
+      there |= 1u << ask;
+    }
+    cp_async_commit();
+    ask = ask + 1 == Ring::kPages ? 0 : ask + 1;
+  };
+  if constexpr (kRing) {
+    for (int i = 0; i < Ring::kPages - 1; ++i) ask_next();
+  } else {
+    now = take(v0 + warp);
+    if (now != 0xFFFFFFFFu) {
+      load_k(f, a, now, h, g, c);
+      load_v(f, a, now, h, g, c);
+    }
   }
 
   // Q fragments: lane (g, c) holds row 8 n + g, dims 32 i + 8 c .. + 8.
@@ -320,14 +381,27 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
   // Page v of the list, pool page `now`; the loads of the next one go out as
   // f's registers come free.
   for (int32_t v = v0 + warp; v < v1; v += kWinWarps) {
-    const uint32_t next = take(v + kWinWarps);
-    if (now == 0xFFFFFFFFu) {  // a bad page: skipped
-      now = next;
-      if (now != 0xFFFFFFFFu) {
-        load_k<D, KV>(f, a, now, h, g, c);
-        load_v<D, KV>(f, a, now, h, g, c);
+    const uint8_t* stage = ring + slot * Ring::kPage;
+    uint32_t next = 0xFFFFFFFFu;
+    if constexpr (kRing) {
+      const bool bad = !((there >> slot) & 1);
+      __syncwarp();  // every lane is through with the place that is asked for next
+      ask_next();
+      cp_async_wait<Ring::kPages - 1>();
+      __syncwarp();  // every lane's part of this page has come
+      slot = slot + 1 == Ring::kPages ? 0 : slot + 1;
+      if (bad) continue;
+      ring_k<D, KV>(f, stage, g, c);
+    } else {
+      next = take(v + kWinWarps);
+      if (now == 0xFFFFFFFFu) {  // a bad page: skipped
+        now = next;
+        if (now != 0xFFFFFFFFu) {
+          load_k(f, a, now, h, g, c);
+          load_v(f, a, now, h, g, c);
+        }
+        continue;
       }
-      continue;
     }
     // ---- S^T = K Q^T
     float x[NT][4];
@@ -384,8 +458,12 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
         for (int e = 0; e < 4; ++e)
           if (e < 2 ? n0 : n1) x[n][e] = NAN;
     }
-    now = next;
-    if (now != 0xFFFFFFFFu) load_k<D, KV>(f, a, now, h, g, c);
+    if constexpr (kRing) {
+      ring_v<D, KV>(f, stage, g, c);
+    } else {
+      now = next;
+      if (now != 0xFFFFFFFFu) load_k(f, a, now, h, g, c);
+    }
     // ---- mask. Most pages are seen whole by every row.
     const int32_t j0 = wp.page(v) * kPageSize;
 #pragma unroll
@@ -555,8 +633,11 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
         }
       }
     }
-    if (now != 0xFFFFFFFFu) load_v<D, KV>(f, a, now, h, g, c);
+    if constexpr (!kRing) {
+      if (now != 0xFFFFFFFFu) load_v(f, a, now, h, g, c);
+    }
   }
+  if constexpr (kRing) __syncthreads();  // the state takes the ring's place
 
   // ---- the warp's state, normalised by its own sum
 #pragma unroll
@@ -690,13 +771,15 @@ static int launch_win_mma_t(const WinArgs& a, int max_pages, int sms, cudaStream
   const int nsplit = win_split(full * a.Hkv, (int64_t)sms * kWinCtas<D, KV, NT>, pages);
   const int64_t blocks = tiles * a.Hkv * nsplit;
   if (blocks > 0x7FFFFFFF) return fail(DD_ERR_INVALID_ARGUMENT, "too many rows");
-  cudaError_t e = cudaSuccess;
-  if (nsplit > 8)
+  using Ring = WinRing<D, KV, NT>;
+  cudaError_t e = cudaFuncSetAttribute(win_mma_kernel<D, KV, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring::kSmem);
+  if (e == cudaSuccess && nsplit > 8)
     e = cudaFuncSetAttribute(win_mma_kernel<D, KV, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(kWinWarps * 32);
+    cfg.dynamicSmemBytes = Ring::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
