@@ -772,7 +772,9 @@ static int launch_win_mma_t(const WinArgs& a, int max_pages, int sms, cudaStream
   const int64_t blocks = tiles * a.Hkv * nsplit;
   if (blocks > 0x7FFFFFFF) return fail(DD_ERR_INVALID_ARGUMENT, "too many rows");
   using Ring = WinRing<D, KV, NT>;
-  cudaError_t e = cudaFuncSetAttribute(win_mma_kernel<D, KV, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring::kSmem);
+  cudaError_t e = cudaSuccess;
+  if (Ring::kSmem > 48 * 1024)
+    e = cudaFuncSetAttribute(win_mma_kernel<D, KV, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring::kSmem);
   if (e == cudaSuccess && nsplit > 8)
     e = cudaFuncSetAttribute(win_mma_kernel<D, KV, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e == cudaSuccess) {
