@@ -135,15 +135,17 @@ int launch_win_simple(const WinArgs& a, cudaStream_t st) {
   return DD_OK;
 }
 
-// Chunks: which of the two tensor-core kernels. Both walk the visible pages of
-// every KV head, the streaming kernel once for 16 rows at about 1.5 ns a page
-// for the whole GPU (two pages' bytes from L2, or HBM), the tcgen05 kernel once
-// for up to 256 rows at 1.9 / 1.9 / 2.15 us (bf16 / E4M3 / MXFP8) for 8 pages on
-// one SM. Measured around the border (streaming, tcgen05; us), windows of 1024,
-// 2048, 4096 tokens: 64 sequences x 4 new tokens, bf16, 4 heads a group 63, 79;
-// x 8 110, 79; E4M3, 8 heads a group x 2 91, 138; x 4 167, 138; MXFP8, 4 heads a
-// group x 4 188, 287; x 8 349, 288; one sequence x 32 27, 75; 4 x 32 E4M3 68, 46.
-static bool tc_is_faster(const WinArgs& a, int max_pages) {
+// Chunks: which of the two tensor-core kernels, and in how many CTAs the tcgen05
+// one splits an item. Both walk the visible pages of every KV head, the streaming
+// kernel once for 16 rows at about 1.5 ns (bf16; FP8 1.1) a page for the whole GPU
+// (two pages' bytes from L2, or HBM), the tcgen05 kernel once for up to 256 rows
+// at 1.9 us (MXFP8 2.15) for 8 pages on one SM, and 8 or 9 us more where shares
+// are joined. Measured around the border (streaming, tcgen05; us), windows of
+// 1024, 2048, 4096 tokens: 64 sequences x 4 new tokens, bf16, 4 heads a group 63,
+// 79; x 8 110, 79; E4M3, 8 heads a group x 2 72, 138; x 4 167, 138; MXFP8, 4 heads
+// a group x 4 152, 287; one sequence x 64, bf16, 18, 24; x 128 26, 24; without a
+// window, 16,000 tokens, x 8 41, 37; x 32 75, 40; x 256 556, 86.
+static bool tc_is_faster(const WinArgs& a, int max_pages, int& nsplit) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const int64_t rows = (int64_t)a.num_rows * a.g, tokens = a.num_rows / a.num_seqs;
@@ -151,9 +153,12 @@ static bool tc_is_faster(const WinArgs& a, int max_pages) {
   if (a.window > 0) pages = std::min(pages, ((int64_t)a.window + a.sinks + tokens) / kPageSize + 2);
   const int64_t tiles16 = std::max<int64_t>(a.num_seqs, (rows + 15) / 16) * a.Hkv;
   const int64_t items = std::max<int64_t>(a.num_seqs, (rows + 255) / 256) * a.Hkv;
+  nsplit = win_tc_split(items, pages, sms);
+  const int64_t tiles = ((pages + 7) / 8 + nsplit - 1) / nsplit;  // of a CTA
   const int64_t tile_ns = a.kv_dtype == DD_DTYPE_MXFP8 ? 2150 : 1900;
-  const int64_t stream_ns = 7000 + tiles16 * pages * 3 / 2;
-  const int64_t tc_ns = (items + sms - 1) / sms * (pages * tile_ns / 8 + 4000);
+  const int64_t join_ns = nsplit == 1 ? 0 : tokens * a.g > 128 ? 9000 : 8000;
+  const int64_t stream_ns = 7000 + tiles16 * pages * (a.kv_dtype == DD_DTYPE_BF16 ? 15 : 11) / 10;
+  const int64_t tc_ns = (items * nsplit + sms - 1) / sms * (tiles * tile_ns + 4000) + join_ns;
   return tc_ns < stream_ns;
 }
 
@@ -208,7 +213,8 @@ static int window_attention(const dd_attn_config* cfg, int32_t num_seqs, int32_t
   const float scale = cfg->scale > 0.f ? cfg->scale : 1.0f / std::sqrt((float)cfg->head_dim);
   a.scale_log2 = scale * kLog2e;
   if (cfg->q_dtype == DD_DTYPE_F32 || cfg->kv_dtype == DD_DTYPE_F32) return launch_win_simple(a, st);
-  if (q_indptr && win_tc_fits(a) && tc_is_faster(a, max_pages)) return launch_win_tc(a, st);
+  int nsplit = 1;
+  if (q_indptr && win_tc_fits(a) && tc_is_faster(a, max_pages, nsplit)) return launch_win_tc(a, nsplit, st);
   return launch_win_mma(a, max_pages, st);
 }
 

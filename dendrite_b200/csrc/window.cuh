@@ -143,10 +143,31 @@ __device__ __forceinline__ void win_tile(const WinArgs& a, int g, int R, int64_t
   tile = (int32_t)max(t - base(lo), (int64_t)-1);
 }
 
+// Another CTA's shared memory: reads at the place that `addr` is in this one's.
+__device__ __forceinline__ float cluster_ld(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 cluster_ld4(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(r) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+
 // Kernel launches (each returns a dd_status).
 int launch_win_simple(const WinArgs& a, cudaStream_t st);
 int launch_win_mma(const WinArgs& a, int max_pages, cudaStream_t st);
 bool win_tc_fits(const WinArgs& a);
-int launch_win_tc(const WinArgs& a, cudaStream_t st);
+int win_tc_split(int64_t items, int64_t pages, int sms);
+int launch_win_tc(const WinArgs& a, int nsplit, cudaStream_t st);
 
 }  // namespace dd

@@ -203,25 +203,6 @@ struct WinShared {
   float cm[NT * 8], cl[NT * 8];       // the CTA's joined state (o[0] holds its output)
 };
 
-__device__ __forceinline__ float cluster_ld(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(r) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 cluster_ld4(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  float4 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(r) : "memory");
-  return v;
-}
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
-}
-
 // CTAs that an SM holds, as far as the registers go. FP8 pages are half the
 // bytes of bf16 ones and need the fourth (128 x 2048 tokens of E4M3: 89 us, in
 // three 97).

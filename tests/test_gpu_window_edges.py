@@ -252,3 +252,34 @@ def test_prompt_between_the_chunks_of_a_batch(cuda):
             cache.layer_prefill(0, q[:17], k[:17], v[:17], [6, 7], 0)
         res.append(cache.layer_chunk(0, q, k, v)[:50])
     assert torch.equal(*res)
+
+
+@pytest.mark.parametrize("shape", [(8, 2, 128, True), (16, 2, 64, False), (12, 1, 128, True)], ids=str)
+@pytest.mark.parametrize("fmt", ["bf16", "e4m3", "mxfp8"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (4096, 4), (3000, 900), (64, 5000)])
+def test_chunks_over_long_sequences(cuda, shape, fmt, window, sinks):
+    """Few rows over many tokens: the tokens are split and joined. One sequence, two, one whose shares are empty for some rows."""
+    Hq, Hkv, D, grouped = shape
+    for tokens, new in (([9001], [100]), ([7000, 5003], [131, 77]), ([6000, 1, 40], [90, 1, 0]), ([130], [130])):
+        b = Batch(43, tokens, new, Hq, Hkv, D, fmt, grouped, window, sinks, dead=10 ** 6)
+        d = Dev(b, cuda)
+        want = b.attention()
+        for mp in (0, 563):
+            status = torch.zeros(2, dtype=torch.int32, device=cuda)
+            out, lse = _run(d, "prefill", max_pages=mp, status=status)
+            assert status.tolist() == [0, 0]
+            check_attention(out, lse, want, f"{shape} {fmt} {new} {mp}", WEIGHTS["prefill"])
+            again, _ = _run(d, "prefill", max_pages=mp)
+            assert torch.equal(out, again)
+
+
+def test_bad_pages_of_a_split_chunk(cuda):
+    for fmt in ("bf16", "e4m3", "mxfp8"):
+        b = Batch(44, [8000], [120], 8, 2, 128, fmt, True, 0, 0)
+        for i in (3, 250, 490):
+            b.ids[i] = b.P + 7
+        d = Dev(b, cuda)
+        status = torch.zeros(2, dtype=torch.int32, device=cuda)
+        out, lse = _run(d, "prefill", status=status)
+        assert status.tolist() == [1, b.P + 7]
+        check_attention(out, lse, b.attention(), fmt, WEIGHTS["prefill"])
