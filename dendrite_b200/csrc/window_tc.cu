@@ -8,13 +8,12 @@
 // window up to its last token's position reach, plus those of the first tokens.
 // The launch has a CTA per item, long ones (late tokens) first. Each CTA that
 // has started (one per SM) claims further ones in place of their starting, as
-// it comes near the end of its item; nothing is planned on the host. Where the
-// items are few, a cluster of 2 to 8 CTAs shares one: each takes some of its
-// tiles, and the outputs are joined through shared memory. (A fixed
+// it comes near the end of its item; nothing is planned on the host. (A fixed
 // share of the items for each CTA took 908 us in place of 799 for 16 chunks of
 // 200 to 2000 tokens, bf16, window 4096, and 291 in place of 270 for 4 chunks of
-// 1000, E4M3, window 2048.) K and V come in tiles of 128 tokens (8 pages of the
-// item's list):
+// 1000, E4M3, window 2048.) Where the items are few, a cluster of 2 to 8 CTAs
+// shares one: each takes some of its tiles, and the outputs are joined through
+// shared memory. K and V come in tiles of 128 tokens (8 pages of the item's list):
 //   softmax      warps 0-3 sub-tile A, 4-7 B, a thread per row: the maximum of
 //                128 scores in TMEM, then the weights of the tile's second and
 //                first 64 tokens, each written over its scores and handed over
@@ -305,10 +304,13 @@ __device__ __forceinline__ void wt_weights(const float (&s)[32], uint64_t sc2, u
   tmem_st16u(taddr, w);
 }
 
-template <int D, int KV>
+// kSplit false: nsplit is 1, known as such (the code of the shares cost the
+// others 1 to 3%).
+template <int D, int KV, bool kSplit>
 __global__ void __maxnreg__((WtCfg<D, KV>::kRegs))
     win_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map, WinArgs a,
-                  int nsplit) {
+                  int cluster) {
+  const int nsplit = kSplit ? cluster : 1;
   using Cfg = WtCfg<D, KV>;
   constexpr bool kFp8 = Cfg::kFp8, kF16 = Cfg::kF16, kHeld = Cfg::kHeld;
   constexpr int kSlots = Cfg::kSlots, kTile = Cfg::kTileBytes, kHalf = Cfg::kHalfBytes;
@@ -979,17 +981,17 @@ int make_kv_tensor_map(CUtensorMap* map, const void* kv, int64_t num_pages, int 
 int make_q_tensor_map(CUtensorMap* map, const void* q, int64_t rows, int64_t row_stride, int Hq, int Hkv, int D,
                       int gqa_map, int tokens);
 
-template <int D, int KV>
+template <int D, int KV, bool kSplit>
 static cudaError_t launch_win_tc_t(const CUtensorMap& kv, const CUtensorMap& q, const WinArgs& a, int32_t units,
                                    int nsplit, cudaStream_t st) {
   using Cfg = WtCfg<D, KV>;
-  cudaError_t e = cudaFuncSetAttribute(win_tc_kernel<D, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
+  cudaError_t e = cudaFuncSetAttribute(win_tc_kernel<D, KV, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem);
   if (e != cudaSuccess) return e;
   if (Cfg::kHeld) {
     // setmaxnreg.inc waits for registers that the block does not have if it
     // was launched with fewer.
     cudaFuncAttributes fa;
-    e = cudaFuncGetAttributes(&fa, win_tc_kernel<D, KV>);
+    e = cudaFuncGetAttributes(&fa, win_tc_kernel<D, KV, kSplit>);
     if (e != cudaSuccess) return e;
     if (fa.numRegs < Cfg::kRegs) return cudaErrorInvalidConfiguration;
   }
@@ -1006,16 +1008,16 @@ static cudaError_t launch_win_tc_t(const CUtensorMap& kv, const CUtensorMap& q, 
   attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = nsplit > 1 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, win_tc_kernel<D, KV>, kv, q, a, nsplit);
+  e = cudaLaunchKernelEx(&cfg, win_tc_kernel<D, KV, kSplit>, kv, q, a, nsplit);
   return e == cudaSuccess ? cudaGetLastError() : e;
 }
-template <int D>
+template <int D, bool kSplit>
 static cudaError_t launch_win_tc_kv(const CUtensorMap& kv, const CUtensorMap& q, const WinArgs& a, int32_t units,
                                     int nsplit, cudaStream_t st) {
   switch (a.kv_dtype) {
-    case DD_DTYPE_BF16: return launch_win_tc_t<D, DD_DTYPE_BF16>(kv, q, a, units, nsplit, st);
-    case DD_DTYPE_E4M3: return launch_win_tc_t<D, DD_DTYPE_E4M3>(kv, q, a, units, nsplit, st);
-    default: return launch_win_tc_t<D, DD_DTYPE_MXFP8>(kv, q, a, units, nsplit, st);
+    case DD_DTYPE_BF16: return launch_win_tc_t<D, DD_DTYPE_BF16, kSplit>(kv, q, a, units, nsplit, st);
+    case DD_DTYPE_E4M3: return launch_win_tc_t<D, DD_DTYPE_E4M3, kSplit>(kv, q, a, units, nsplit, st);
+    default: return launch_win_tc_t<D, DD_DTYPE_MXFP8, kSplit>(kv, q, a, units, nsplit, st);
   }
 }
 
@@ -1048,8 +1050,9 @@ int launch_win_tc(const WinArgs& a, int nsplit, cudaStream_t st) {
   if (!rc) rc = make_q_tensor_map(&q, a.q, a.num_rows, a.q_stride, a.Hq, a.Hkv, a.D, a.gqa_map, 128 / a.g);
   if (rc) return rc;
   const int32_t units = (int32_t)win_tc_units(a);
-  const cudaError_t e = a.D == 64 ? launch_win_tc_kv<64>(kv, q, a, units, nsplit, st)
-                                  : launch_win_tc_kv<128>(kv, q, a, units, nsplit, st);
+  const auto launch = a.D == 64 ? (nsplit > 1 ? launch_win_tc_kv<64, true> : launch_win_tc_kv<64, false>)
+                                : (nsplit > 1 ? launch_win_tc_kv<128, true> : launch_win_tc_kv<128, false>);
+  const cudaError_t e = launch(kv, q, a, units, nsplit, st);
   if (e != cudaSuccess) return fail(DD_ERR_CUDA, std::string("window attention launch: ") + cudaGetErrorString(e));
   return DD_OK;
 }
