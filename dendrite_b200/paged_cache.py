@@ -115,6 +115,11 @@ class PagedKVCache:
         indptr = np.ascontiguousarray(indptr, dtype=np.int32)
         block_ids = np.ascontiguousarray(block_ids, dtype=np.uint32)
         pos = np.ascontiguousarray(positions, dtype=np.int64)
+        # The plan checks the lengths against the tables; a step of windowed layers has none.
+        self._check_tables(indptr, block_ids)
+        if len(pos) != len(indptr) - 1 or np.any(pos < 0) or \
+                np.any(pos >= np.diff(indptr).astype(np.int64) * PAGE_SIZE):
+            raise _lib.InvalidArgument("the tables and the positions do not fit together")
         ntok = (pos + 1).astype(np.int32)
         blk = block_ids[indptr[:-1] + pos // PAGE_SIZE]
         advanced = False
@@ -138,10 +143,14 @@ class PagedKVCache:
         self._tables = (indptr.copy(), block_ids.copy())
         return advanced
 
+    @staticmethod
+    def _check_tables(indptr, block_ids) -> None:
+        if len(indptr) < 1 or indptr[0] < 0 or np.any(np.diff(indptr) < 0) or indptr[-1] > len(block_ids):
+            raise _lib.InvalidArgument("the tables and the block ids do not fit together")
+
     def _device_tables(self, indptr, block_ids, ntok):
         """(page_indptr, page_indices, num_tokens on the device, pages of the longest table)."""
-        if indptr[0] < 0 or np.any(np.diff(indptr) < 0) or indptr[-1] > len(block_ids):
-            raise _lib.InvalidArgument("the tables and the block ids do not fit together")
+        self._check_tables(indptr, block_ids)
         dev = [torch.from_numpy(np.ascontiguousarray(x).view(np.int32)).to(self.device)
                for x in (indptr, block_ids, ntok)]
         return (*dev, int(np.diff(indptr).max(initial=0)))

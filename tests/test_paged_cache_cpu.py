@@ -1,0 +1,38 @@
+"""PagedKVCache's own checks and bookkeeping, without a GPU (no kernel runs)."""
+import numpy as np
+import pytest
+import torch
+
+import dendrite_b200 as dd
+
+HQ, HKV, D, P = 4, 2, 64, 8
+
+
+def _cache(windows):
+    return dd.PagedKVCache(len(windows), P, HQ, HKV, D, device="cpu", windows=windows)
+
+
+@pytest.mark.parametrize("windows", [[None], [(20, 2)], [(20, 2), None]], ids=["full", "windowed", "both"])
+@pytest.mark.parametrize("indptr,ids,positions", [
+    ([0, 1, 2], [3, 5], [16, 0]),            # past the first table: the place is the second sequence's
+    ([0, 1, 2], [3, 5], [0, 16]),            # past the last one
+    ([0, 1, 2], [3, 5], [0, -1]),            # before the first token
+    ([0, 1, 2], [3, 5], [0, 2 ** 32]),       # a position that 32 bits would cut off to 0
+    ([0, 0, 1], [3], [0, 0]),                # a sequence without a page
+    ([0, 1, 2], [3, 5], [0]),                # fewer positions than tables
+    ([0, 1, 3], [3, 5], [0, 20]),            # tables past the ids
+    ([0, 2, 1], [3, 5], [0, 0]),
+    ([-1, 1, 2], [3, 5], [0, 0]),
+    ([], [], []),
+], ids=str)
+def test_a_step_outside_its_tables_is_refused(windows, indptr, ids, positions):
+    with pytest.raises(dd.InvalidArgument, match="fit together"):
+        _cache(windows).begin_step(np.array(indptr, np.int32), np.array(ids, np.uint32), positions)
+
+
+def test_a_step_stores_at_its_positions():
+    cache = _cache([(20, 2)])
+    assert cache.begin_step([0, 2, 2 + 1], [3, 5, 1], [17, 15]) is False
+    assert cache._page_ids.tolist() == [5, 1] and cache._slots.tolist() == [1, 15]
+    ip, ids, ntok, longest = cache._step
+    assert (ip.tolist(), ids.tolist(), ntok.tolist(), longest) == ([0, 2, 3], [3, 5, 1], [18, 16], 2)
