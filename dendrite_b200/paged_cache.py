@@ -113,7 +113,7 @@ class PagedKVCache:
         previous tables unless the caller says so with tree_grew_only=True —
         and re-planned otherwise. Returns True when advanced."""
         indptr = np.ascontiguousarray(indptr, dtype=np.int32)
-        block_ids = np.ascontiguousarray(block_ids, dtype=np.uint32)
+        block_ids = np.ascontiguousarray(np.asarray(block_ids).astype(np.uint32))  # -1: a page given back
         pos = np.ascontiguousarray(positions, dtype=np.int64)
         # The plan checks the lengths against the tables; a step of windowed layers has none.
         self._check_tables(indptr, block_ids)

@@ -36,3 +36,13 @@ def test_a_step_stores_at_its_positions():
     assert cache._page_ids.tolist() == [5, 1] and cache._slots.tolist() == [1, 15]
     ip, ids, ntok, longest = cache._step
     assert (ip.tolist(), ids.tolist(), ntok.tolist(), longest) == ([0, 2, 3], [3, 5, 1], [18, 16], 2)
+
+
+@pytest.mark.parametrize("ids", [[-1, 4], np.array([-1, 4]), np.array([-1, 4], np.int32),
+                                 np.array([2 ** 32 - 1, 4], np.uint32)], ids=["list", "int64", "int32", "uint32"])
+def test_a_step_over_pages_given_back(ids):
+    """A table entry of a page that no window reaches any more may be -1, in whatever type the ids come."""
+    cache = _cache([(4, 0)])
+    cache.begin_step([0, 2], ids, [30])
+    assert cache._page_ids.tolist() == [4] and cache._slots.tolist() == [14]
+    assert cache._step[1].tolist() == [-1, 4]
