@@ -123,24 +123,24 @@ class PagedKVCache:
         ntok = (pos + 1).astype(np.int32)
         blk = block_ids[indptr[:-1] + pos // PAGE_SIZE]
         advanced = False
+        if not all(self.windows):  # else nothing needs the plan
+            if self.plan is not None and self._ntok is not None and len(self._ntok) == len(ntok) \
+                    and np.array_equal(self._ntok + 1, ntok) \
+                    and (tree_grew_only or (tree_grew_only is None and self._only_grew(indptr, block_ids))):
+                advanced = self.plan.advance(np.ones(len(ntok), np.int32), blk)
+            if not advanced:
+                if self.plan is None:
+                    self.plan = CascadePlan(self.cfg, indptr, block_ids, ntok)
+                else:
+                    self.plan.rebuild(indptr, block_ids, ntok)
+            self.plan.upload(self.device)
+            self._ntok = ntok
+            self._tables = (indptr.copy(), block_ids.copy())
+        # Only now: a step that the plan refuses leaves the last one as it was.
         if any(self.windows):
             self._step = self._device_tables(indptr, block_ids, ntok)
         self._page_ids = torch.from_numpy(blk.astype(np.int32)).to(self.device)
         self._slots = torch.from_numpy((pos % PAGE_SIZE).astype(np.int32)).to(self.device)
-        if all(self.windows):  # nothing needs the plan
-            return advanced
-        if self.plan is not None and self._ntok is not None and len(self._ntok) == len(ntok) \
-                and np.array_equal(self._ntok + 1, ntok) \
-                and (tree_grew_only or (tree_grew_only is None and self._only_grew(indptr, block_ids))):
-            advanced = self.plan.advance(np.ones(len(ntok), np.int32), blk)
-        if not advanced:
-            if self.plan is None:
-                self.plan = CascadePlan(self.cfg, indptr, block_ids, ntok)
-            else:
-                self.plan.rebuild(indptr, block_ids, ntok)
-        self.plan.upload(self.device)
-        self._ntok = ntok
-        self._tables = (indptr.copy(), block_ids.copy())
         return advanced
 
     @staticmethod

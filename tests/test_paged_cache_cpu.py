@@ -46,3 +46,28 @@ def test_a_step_over_pages_given_back(ids):
     cache.begin_step([0, 2], ids, [30])
     assert cache._page_ids.tolist() == [4] and cache._slots.tolist() == [14]
     assert cache._step[1].tolist() == [-1, 4]
+
+
+def test_a_refused_step_leaves_the_last_one(monkeypatch):
+    """When the plan refuses a step, nothing of it stays: the pages that the layers write and the
+    tables that windowed layers read are still those of the plan that is in place."""
+    import dendrite_b200.paged_cache as pc
+
+    class Plan:
+        def __init__(self, cfg, indptr, ids, ntok):
+            self.built = list(ids)
+
+        def rebuild(self, indptr, ids, ntok):
+            raise dd.InvalidArgument("refused")
+
+        def upload(self, device):
+            pass
+
+    monkeypatch.setattr(pc, "CascadePlan", Plan)
+    cache = _cache([(20, 2), None])
+    cache.begin_step([0, 1], [3], [4])
+    with pytest.raises(dd.InvalidArgument, match="refused"):
+        cache.begin_step([0, 1], [6], [9])
+    assert cache.plan.built == [3]
+    assert cache._page_ids.tolist() == [3] and cache._slots.tolist() == [4]
+    assert cache._step[1].tolist() == [3] and cache._step[2].tolist() == [5]
