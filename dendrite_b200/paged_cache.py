@@ -132,7 +132,12 @@ class PagedKVCache:
                 if self.plan is None:
                     self.plan = CascadePlan(self.cfg, indptr, block_ids, ntok)
                 else:
-                    self.plan.rebuild(indptr, block_ids, ntok)
+                    try:
+                        self.plan.rebuild(indptr, block_ids, ntok)
+                    except _lib.InvalidArgument:  # which empties the plan
+                        self.plan.rebuild(*self._tables, self._ntok)
+                        self.plan.upload(self.device)
+                        raise
             self.plan.upload(self.device)
             self._ntok = ntok
             self._tables = (indptr.copy(), block_ids.copy())

@@ -49,25 +49,21 @@ def test_a_step_over_pages_given_back(ids):
 
 
 def test_a_refused_step_leaves_the_last_one(monkeypatch):
-    """When the plan refuses a step, nothing of it stays: the pages that the layers write and the
-    tables that windowed layers read are still those of the plan that is in place."""
-    import dendrite_b200.paged_cache as pc
-
-    class Plan:
-        def __init__(self, cfg, indptr, ids, ntok):
-            self.built = list(ids)
-
-        def rebuild(self, indptr, ids, ntok):
-            raise dd.InvalidArgument("refused")
-
-        def upload(self, device):
-            pass
-
-    monkeypatch.setattr(pc, "CascadePlan", Plan)
+    """When the plan refuses a step, nothing of it stays: the pages that the layers write, the tables
+    that windowed layers read and the plan are those of the last step, and the next one goes on from it."""
+    uploads = []
+    monkeypatch.setattr(dd.CascadePlan, "upload", lambda plan, device=None, stream=None: uploads.append(plan.batch_size))
     cache = _cache([(20, 2), None])
-    cache.begin_step([0, 1], [3], [4])
-    with pytest.raises(dd.InvalidArgument, match="refused"):
-        cache.begin_step([0, 1], [6], [9])
-    assert cache.plan.built == [3]
-    assert cache._page_ids.tolist() == [3] and cache._slots.tolist() == [4]
-    assert cache._step[1].tolist() == [3] and cache._step[2].tolist() == [5]
+    cache.begin_step([0, 1, 2], [3, 5], [4, 7])
+    nodes = {k: v.tolist() for k, v in cache.plan.nodes().items()}
+    with pytest.raises(dd.InvalidArgument):
+        cache.begin_step([0, 1], [P + 92], [9])         # no such page
+    assert cache._page_ids.tolist() == [3, 5] and cache._slots.tolist() == [4, 7]
+    assert cache._step[1].tolist() == [3, 5] and cache._step[2].tolist() == [5, 8]
+    assert cache.plan.batch_size == 2 and {k: v.tolist() for k, v in cache.plan.nodes().items()} == nodes
+    assert cache.begin_step([0, 1, 2], [3, 5], [5, 8]) is True
+    assert uploads == [2, 2, 2]
+    cache = _cache([(20, 2), None])
+    with pytest.raises(dd.InvalidArgument):
+        cache.begin_step([0, 1], [P + 92], [9])
+    assert cache.plan is None and cache._step is None and cache._page_ids is None
