@@ -160,8 +160,17 @@ class PagedKVCache:
                for x in (indptr, block_ids, ntok)]
         return (*dev, int(np.diff(indptr).max(initial=0)))
 
+    @staticmethod
+    def _check_rows(q, k, v, rows) -> None:
+        """The append takes a page and a slot for each row of K."""
+        if not q.shape[0] == k.shape[0] == v.shape[0] == rows:
+            raise _lib.InvalidArgument(f"q, k and v must have the batch's {rows} rows")
+
     def layer_step(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         """Store layer `layer`'s new K/V [B, Hkv, D] and attend with q [B, Hq, D]."""
+        if self._page_ids is None:
+            raise _lib.InvalidArgument("begin_step first")
+        self._check_rows(q, k, v, len(self._page_ids))
         append_kv_batch(self.cfg, self.pools[layer], self.scales[layer], self._page_ids, self._slots,
                         k.contiguous(), v.contiguous())
         q = q.to(torch.bfloat16).contiguous()
@@ -183,6 +192,9 @@ class PagedKVCache:
         causal attention of q [S, Hq, D] (new token i sees tokens
         0 .. prefix_len + i)."""
         S = q.shape[0]
+        self._check_rows(q, k, v, S)
+        if prefix_len < 0 or prefix_len + S > len(table) * PAGE_SIZE:
+            raise _lib.InvalidArgument("the table, prefix_len and the rows do not fit together")
         if self.windows[layer]:
             tbl = np.asarray(table).astype(np.uint32)
             return self._chunk(layer, self._chunk_tables([0, len(tbl)], tbl, [prefix_len + S], [S]), q, k, v)

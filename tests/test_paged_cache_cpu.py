@@ -67,3 +67,35 @@ def test_a_refused_step_leaves_the_last_one(monkeypatch):
     with pytest.raises(dd.InvalidArgument):
         cache.begin_step([0, 1], [P + 92], [9])
     assert cache.plan is None and cache._step is None and cache._page_ids is None
+
+
+def _rows(n, heads):
+    return torch.zeros(n, heads, D, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("windows", [[None], [(20, 2)]], ids=["full", "windowed"])
+@pytest.mark.parametrize("nq,nk,nv", [(2, 3, 3), (3, 2, 2), (2, 2, 1), (2, 1, 2), (3, 3, 3), (1, 1, 1)], ids=str)
+def test_rows_that_are_not_the_steps(monkeypatch, windows, nq, nk, nv):
+    """The append reads a page and a slot for each row of K: more rows than the step has would read past them."""
+    monkeypatch.setattr(dd.CascadePlan, "upload", lambda plan, device=None, stream=None: None)
+    cache = _cache(windows)
+    with pytest.raises(dd.InvalidArgument, match="begin_step"):
+        cache.layer_step(0, _rows(2, HQ), _rows(2, HKV), _rows(2, HKV))
+    cache.begin_step([0, 1, 2], [3, 5], [4, 7])
+    with pytest.raises(dd.InvalidArgument, match="2 rows"):
+        cache.layer_step(0, _rows(nq, HQ), _rows(nk, HKV), _rows(nv, HKV))
+
+
+@pytest.mark.parametrize("windows", [[None], [(20, 2)]], ids=["full", "windowed"])
+@pytest.mark.parametrize("nk,nv", [(3, 3), (1, 1), (2, 1), (1, 2)], ids=str)
+def test_rows_that_are_not_the_prompts(windows, nk, nv):
+    with pytest.raises(dd.InvalidArgument, match="2 rows"):
+        _cache(windows).layer_prefill(0, _rows(2, HQ), _rows(nk, HKV), _rows(nv, HKV), [3], 4)
+
+
+@pytest.mark.parametrize("windows", [[None], [(20, 2)]], ids=["full", "windowed"])
+@pytest.mark.parametrize("table,prefix", [([3], 15), ([3], -1), ([], 0)], ids=str)
+def test_a_prompt_outside_its_table(windows, table, prefix):
+    """Position -1 would be the last slot of the table's last page."""
+    with pytest.raises(dd.InvalidArgument, match="fit together"):
+        _cache(windows).layer_prefill(0, _rows(2, HQ), _rows(2, HKV), _rows(2, HKV), table, prefix)
