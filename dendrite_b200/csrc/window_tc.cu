@@ -9,9 +9,9 @@
 // The launch has a CTA per item, long ones (late tokens) first. Each CTA that
 // has started (one per SM) claims further ones in place of their starting, as
 // it comes near the end of its item; nothing is planned on the host. (A fixed
-// share of the items for each CTA took 908 us in place of 799 for 16 chunks of
-// 200 to 2000 tokens, bf16, window 4096, and 291 in place of 270 for 4 chunks of
-// 1000, E4M3, window 2048.) Where the items are few, a cluster of 2 to 8 CTAs
+// share of the items for each CTA took 291 us in place of 270 for 4 chunks of 1000
+// tokens, E4M3, window 2048, and with weights of one bf16 term 908 in place of 799
+// for 16 chunks of 200 to 2000, bf16, window 4096.) Where the items are few, a cluster of 2 to 8 CTAs
 // shares one: each takes some of its tiles, and the outputs are joined through
 // shared memory. K and V come in tiles of 128 tokens (8 pages of the item's list):
 //   softmax      warps 0-3 sub-tile A, 4-7 B, a thread per row: the maximum of
@@ -26,18 +26,18 @@
 //                (finding an item is a chain of dependent loads and divisions),
 //                and an item's Q once the previous item's last scores are done
 // The tensor core works on one sub-tile while the softmax of the other runs.
-// A tile of 256 rows is 2080 cycles of products at D = 128 (65 each, their
-// shared-memory operands keeping that memory busy throughout) and 2048 of
-// exponentials.
+// A tile of 256 rows at D = 128 is 3120 cycles of products (65 each, their
+// shared-memory operands keeping that memory busy throughout; E4M3, whose weights
+// are one term, 2080) and 2048 of exponentials.
 //
 // Types. bf16 and MXFP8 pages take bf16 products; a code times its power of
 // two is exact in bf16. E4M3 pages take f16 products on the bare codes (exact,
 // one conversion for two codes): Q's rows are scaled by a power of two into
 // f16's range and the per-head scales go into the score scale and the epilogue.
-// The softmax weights are rounded once (to nearest) to the products' type, 8
-// bits in bf16 and 11 in f16: a second bf16 term would cost half as many
-// products again, and the output is rounded to bf16's 8 bits anyway. Row sums
-// and references are f32.
+// The softmax weights are two bf16 terms (16 bits, as in the streaming kernel and
+// the plans' kernels: with one, 1.1e-3 off on average, a prompt of 8191 tokens takes
+// 394 us in place of 495) or one f16 term, rounded to nearest (11 bits, 2^-32 of the
+// largest weight at worst). Row sums and references are f32.
 //
 // Masks. The item's page list is a virtual axis x (first-token pages, then
 // window pages); a row of position p sees x in [p - window + 1 - shift, p -
@@ -70,8 +70,9 @@ struct WtCfg {
   static constexpr int kThreads = 32 * (kProducer + 4);
   // FP8: the softmax takes registers over from the other warps and holds a
   // tile's scores, in place of reading their first half again (8 chunks of 200
-  // to 700 tokens, window 1024, MXFP8: 96 us -> 92; 4 of 1000, window 2048,
-  // E4M3: 309 -> 306; bf16, 8191 tokens, window 4096: 384 -> 391, so not there).
+  // to 700 tokens, window 1024, MXFP8: 109 us -> 102; 4 of 1000, window 2048,
+  // E4M3: 309 -> 306; bf16, 16 of 200 to 2000, window 4096: 1011 -> 1013, 64 of 16:
+  // 285 -> 296, so not there).
   // Together no more than the block's at launch.
   static constexpr bool kHeld = kFp8;
   static constexpr int kRegs = kFp8 ? 128 : 168, kRegsSoftmax = 184, kRegsConvert = 80, kRegsRest = 64;
@@ -275,6 +276,12 @@ __device__ __forceinline__ void store16(uint16_t* out, const uint32_t (&w)[16], 
   }
 }
 
+__device__ __forceinline__ void tmem_st8u(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // This thread's O row times f (rare: kept small rather than fast).
 template <int D>
 __device__ __forceinline__ void wt_rescale(uint32_t taddr, float f) {
@@ -290,18 +297,26 @@ __device__ __forceinline__ void wt_rescale(uint32_t taddr, float f) {
   tmem_wait_st();
 }
 
-// Weights of 32 scores, to the products' type; their f32 sum is added to acc.
+// Weights of 32 scores, to the products' type (bf16: the second terms 32 columns
+// on); their f32 sum is added to acc.
 template <bool kF16>
 __device__ __forceinline__ void wt_weights(const float (&s)[32], uint64_t sc2, uint64_t nm2, uint64_t& acc, uint32_t taddr) {
-  uint32_t w[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint64_t x = f2_fma(f2_pack(s[2 * i], s[2 * i + 1]), sc2, nm2);
-    const uint64_t e = f2_pack(fast_exp2(f2_lo(x)), fast_exp2(f2_hi(x)));
-    acc = f2_add(acc, e);
-    w[i] = kF16 ? pack_f16x2(f2_lo(e), f2_hi(e)) : pack_bf16x2(f2_lo(e), f2_hi(e));
+  for (int j = 0; j < 32; j += 16) {  // eight columns at a time: sixteen cost registers (MXFP8 chunks 107 us, 102)
+    uint32_t w[8], lo[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint64_t x = f2_fma(f2_pack(s[j + 2 * i], s[j + 2 * i + 1]), sc2, nm2);
+      const uint64_t e = f2_pack(fast_exp2(f2_lo(x)), fast_exp2(f2_hi(x)));
+      acc = f2_add(acc, e);
+      if constexpr (kF16)
+        w[i] = pack_f16x2(f2_lo(e), f2_hi(e));
+      else
+        split_bf16x2_packed(e, w[i], lo[i]);
+    }
+    tmem_st8u(taddr + j / 2, w);
+    if constexpr (!kF16) tmem_st8u(taddr + 32 + j / 2, lo);
   }
-  tmem_st16u(taddr, w);
 }
 
 // kSplit false: nsplit is 1, known as such (the code of the shares cost the
@@ -639,8 +654,9 @@ __global__ void __maxnreg__((WtCfg<D, KV>::kRegs))
         const bool clean = (pages & 0xffu) == 0xffu && wt_whole(a, it, x0, kTcTok);
         // Two chunks at a time, both read before the first is stored: no load
         // may pass a store that could be to its address, so one at a time each
-        // waits for the one before (the calls named at kHeld: MXFP8 92 us
-        // -> 84, E4M3 306 -> 292, as long as without any widening; four: 84, 295).
+        // waits for the one before (the calls named at kHeld, with weights of one
+        // term: MXFP8 92 us -> 84, E4M3 306 -> 292, as long as without any widening;
+        // four: 84, 295).
         constexpr int kBatch = 2;
 #pragma unroll 1
         for (int i0 = 0; i0 < kChunks / kConvThreads; i0 += kBatch) {
@@ -815,15 +831,19 @@ __global__ void __maxnreg__((WtCfg<D, KV>::kRegs))
           const int vi = g0 + 2 * j + 1, ki = vi + 1, slot = vi % kSlots;
           const uint32_t o = tb + col_o(x), p = tb + col_s(x), v = s_addr + (slot * kTile >> 4);
           const bool two = 2 * j + 1 < nchunks, more = j + 1 < ntiles;
+          auto product = [&](uint32_t pt, uint32_t vt, uint32_t acc) {  // of 64 tokens; bf16: of both terms
+            umma_pv<Cfg::kIdPV>(o, pt, vt, kHalf >> 4, acc);
+            if constexpr (!kF16) umma_pv<Cfg::kIdPV>(o, pt + 32, vt, kHalf >> 4, 1u);
+          };
           ok = wait(&bars.kv_full[slot], vi / kSlots) && (!more || wait(&bars.kv_full[ki % kSlots], ki / kSlots));
           if (two) {
             ok = ok && wait(&bars.p_full[x][1], used[1]++);
             if (!ok) break;
-            umma_pv<Cfg::kIdPV>(o, p + kWtChunk, v + (kWtChunk * 128 >> 4), kHalf >> 4, j > 0 ? 1u : 0u);
+            product(p + kWtChunk, v + (kWtChunk * 128 >> 4), j > 0 ? 1u : 0u);
           }
           ok = ok && my_turn() && wait(&bars.p_full[x][0], used[0]++);
           if (!ok) break;
-          umma_pv<Cfg::kIdPV>(o, p, v, kHalf >> 4, j > 0 || two ? 1u : 0u);
+          product(p, v, j > 0 || two ? 1u : 0u);
           umma_commit_one(&bars.kv_empty[slot]);
           if (more)
             issue_qk(j + 1);
