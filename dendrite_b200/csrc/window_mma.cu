@@ -22,17 +22,19 @@
 //  - S^T and O^T have their query row in the same lane, so the softmax state
 //    (reference, sum) and a rescale need no exchange; the reference moves only
 //    when a score passes it by 8 (log2 units), found by one vote a page.
-//  - FP8 codes are exact in f16, so FP8 pages take f16 products on the codes
-//    themselves: a row of Q is scaled by a power of two into f16's range, the
-//    per-head E4M3 scales are folded into the score scale and the epilogue,
-//    MXFP8's exponents of K scale S per 32-dim block, those of V scale the
-//    weights per block, relative to the largest exponent seen so far.
+//  - FP8 codes are exact in f16, so the scores take f16 products on the codes
+//    themselves: a row of Q is scaled by a power of two into f16's range, E4M3's
+//    per-head scale is folded into the score scale, MXFP8's exponents of K scale
+//    S per 32-dim block. E4M3's V is taken the same way, its scale in the
+//    epilogue. MXFP8's V is widened to bf16, where a code times its power of two
+//    is exact whatever the other tokens' exponents are.
 //  - The warps of a CTA take pages in turn, the CTAs of a cluster (1 to 16)
 //    split the visible pages; the states are joined through shared memory and
 //    the cluster's shared memory, so a call is one launch without workspace.
-// Weights are rounded to two bf16 terms for bf16 pages (bf16's products take
-// both operands in bf16; two terms keep 16 bits) and to f16 for FP8 pages (11
-// bits, 2^-32 of the largest weight at worst); sums and references are f32.
+// Weights are rounded to two bf16 terms for bf16 and MXFP8 pages (bf16's products
+// take both operands in bf16; two terms keep 16 bits) and to f16 for E4M3 pages
+// (11 bits, 2^-32 of the largest weight at worst, V of a head having one scale);
+// sums and references are f32.
 #include <algorithm>
 
 #include "window.cuh"
@@ -85,8 +87,8 @@ template <int D, int KV>
 struct WinFrag {
   uint2 k[D / 32][2];
   uint32_t v[D / 32][4];
-  // MXFP8: exponent bytes of tokens g, g + 8 (D / 32 of them each)
-  uint32_t ek[2][(D + 127) / 128], ev[2][(D + 127) / 128];
+  // MXFP8: exponent bytes (D / 32 of them each) of K's tokens g, g + 8 and V's tokens t(j)
+  uint32_t ek[2][(D + 127) / 128], ev[4][(D + 127) / 128];
 };
 
 // ---- bf16: straight from global memory.
@@ -177,8 +179,8 @@ __device__ __forceinline__ void ring_v(WinFrag<D, KV>& f, const uint8_t* stage, 
                                                      ring_unit<D>(2 * c + (j & 1) + 8 * (j >> 1), i) * 32 + 4 * g);
   if constexpr (KV == kWinMx) {
     const uint8_t* e = stage + 2 * kPageSize * D + kPageSize * (D / 32);
-    ring_exps<D>(e + g * (D / 32), f.ev[0]);
-    ring_exps<D>(e + (g + 8) * (D / 32), f.ev[1]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ring_exps<D>(e + (2 * c + (j & 1) + 8 * (j >> 1)) * (D / 32), f.ev[j]);
   }
 }
 // Byte b of a word of E8M0 exponents as a power of two (0: 0 in place of
@@ -192,6 +194,21 @@ __device__ __forceinline__ bool has_nan_exp(const uint32_t (&e)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) any |= (~e[i] - 0x01010101u) & e[i] & 0x80808080u;  // a zero byte of ~e
   return any != 0;
+}
+// Byte b of two words of E8M0 exponents as a bf16 pair of powers of two (0: 2^-127; 255: infinity).
+__device__ __forceinline__ uint32_t exp_pair(uint32_t w0, uint32_t w1, int b) {
+  return __vmaxu2((__byte_perm(w0, w1, b | (b + 4) << 8) & 0xff00ffu) << 7, 0x00400040u);
+}
+// Four E4M3 codes (a word) as two bf16 pairs, exact, each pair times `by`.
+__device__ __forceinline__ void e4m3x4_bf16_by(uint32_t codes, uint32_t by, uint32_t& lo, uint32_t& hi) {
+  const float2 a = e4m3x2_to_float2((uint16_t)(codes & 0xffffu)), b = e4m3x2_to_float2((uint16_t)(codes >> 16));
+  auto times = [&](float2 x) {
+    const uint32_t w = pack_bf16x2(x.x, x.y);
+    const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(&by));
+    return *reinterpret_cast<const uint32_t*>(&y);
+  };
+  lo = times(a);
+  hi = times(b);
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 __device__ __forceinline__ uint32_t word(const uint2& v, int i) { return i == 0 ? v.x : v.y; }
@@ -223,7 +240,8 @@ struct WinRing {
 template <int D, int KV, int NT>
 __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_kernel(WinArgs a, int nsplit) {
   constexpr int R = NT * 8;
-  constexpr bool kF16 = KV != kWinBf16;
+  constexpr bool kF16 = KV != kWinBf16;    // Q, K
+  constexpr bool kF16V = KV == kWinE4m3;  // weights, V
   constexpr int kBlocks = D / 32;
   using Ring = WinRing<D, KV, NT>;
   constexpr bool kRing = Ring::kUsed;
@@ -355,9 +373,6 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[n][i][e] = 0.f;
   }
-  uint32_t ref_e[(D + 127) / 128];  // MXFP8: largest exponent of V so far, per 32-dim block
-#pragma unroll
-  for (int i = 0; i < (D + 127) / 128; ++i) ref_e[i] = 0;
 
   // Page v of the list, pool page `now`; the loads of the next one go out as
   // f's registers come free.
@@ -472,19 +487,25 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
           } else {
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) f.v[i][j] = 0;
+            if constexpr (KV == kWinMx) {
+#pragma unroll
+              for (int i = 0; i < (D + 127) / 128; ++i) f.ev[j][i] = 0;
+            }
           }
         }
       }
-      if constexpr (KV == kWinMx) {
+    }
+    if constexpr (KV == kWinMx) {
+      // exp_pair takes the NaN exponent for infinity: NaN codes make it NaN.
+      bool some = false;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int32_t t = j0 + g + 8 * half;
-          const bool seen = t <= p_hi && (a.window == 0 || t > p_lo - a.window || t < a.sinks);
-          if (!seen) {
+      for (int j = 0; j < 4; ++j) some |= has_nan_exp(f.ev[j]);
+      if (__any_sync(0xffffffffu, some)) {
 #pragma unroll
-            for (int i = 0; i < (D + 127) / 128; ++i) f.ev[half][i] = 0;
-          }
-        }
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < kBlocks; ++i)
+            if (((f.ev[j][i / 4] >> (8 * (i % 4))) & 255) == 255) f.v[i][j] = 0x7f7f7f7f;
       }
     }
     // ---- references: moved for all rows once some score passes its own by
@@ -513,104 +534,69 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
           }
         }
     }
-    if constexpr (KV == kWinMx) {
-      bool up = false;
-#pragma unroll
-      for (int i = 0; i < (D + 127) / 128; ++i)
-        up |= __vmaxu4(__vmaxu4(f.ev[0][i], f.ev[1][i]), ref_e[i]) != ref_e[i];
-      if (__any_sync(0xffffffffu, up)) {
-#pragma unroll
-        for (int i = 0; i < (D + 127) / 128; ++i) {
-          uint32_t t = __vmaxu4(f.ev[0][i], f.ev[1][i]);
-#pragma unroll
-          for (int b = 4; b < 32; b <<= 1) t = __vmaxu4(t, __shfl_xor_sync(0xffffffffu, t, b));
-          t = __vmaxu4(t, ref_e[i]);
-#pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            if (4 * i + b < kBlocks) {
-              const int down = (int)((t >> (8 * b)) & 255) - (int)((ref_e[i] >> (8 * b)) & 255);
-              const float by = down > 126 ? 0.f : __uint_as_float((uint32_t)(127 - down) << 23);
-#pragma unroll
-              for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  o[n][2 * (4 * i + b)][e] *= by;
-                  o[n][2 * (4 * i + b) + 1][e] *= by;
-                }
-            }
-          }
-          ref_e[i] = t;
-        }
-      }
-    }
     // ---- weights
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float ref = (m[n][e] == -INFINITY ? 0.f : m[n][e]) - (kF16 ? kWinF16Shift : 0.f);
+        const float ref = (m[n][e] == -INFINITY ? 0.f : m[n][e]) - (kF16V ? kWinF16Shift : 0.f);
         x[n][e] = fast_exp2(x[n][e] - ref);
         x[n][e + 2] = fast_exp2(x[n][e + 2] - ref);
         l[n][e] += x[n][e] + x[n][e + 2];
       }
     }
     // ---- O^T += V^T P^T
-    if constexpr (KV == kWinBf16) {
-      uint32_t hi[NT][2], lo[NT][2];
+    uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+      for (int half = 0; half < 2; ++half) {
+        if constexpr (kF16V) {
+          hi[n][half] = movm_trans(pack_f16x2(x[n][2 * half], x[n][2 * half + 1]));
+        } else {
           uint32_t a_hi, a_lo;
           split_bf16x2(x[n][2 * half], x[n][2 * half + 1], a_hi, a_lo);
           hi[n][half] = movm_trans(a_hi);
           lo[n][half] = movm_trans(a_lo);
         }
+      }
+    auto product = [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        win_mma<kF16V>(o[n][i], a0, a1, a2, a3, hi[n][0], hi[n][1]);
+        if constexpr (!kF16V) win_mma<false>(o[n][i], a0, a1, a2, a3, lo[n][0], lo[n][1]);
+      }
+    };
+    if constexpr (KV == kWinBf16) {
 #pragma unroll
       for (int i = 0; i < D / 64; ++i)
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const uint32_t w0 = word(f.v[i][0], u), w1 = word(f.v[i][1], u), w2 = word(f.v[i][2], u), w3 = word(f.v[i][3], u);
-          const uint32_t a0 = __byte_perm(w0, w1, 0x5410), a1 = __byte_perm(w0, w1, 0x7632);
-          const uint32_t a2 = __byte_perm(w2, w3, 0x5410), a3 = __byte_perm(w2, w3, 0x7632);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            win_mma<false>(o[n][4 * i + u], a0, a1, a2, a3, hi[n][0], hi[n][1]);
-            win_mma<false>(o[n][4 * i + u], a0, a1, a2, a3, lo[n][0], lo[n][1]);
-          }
+          product(4 * i + u, __byte_perm(w0, w1, 0x5410), __byte_perm(w0, w1, 0x7632), __byte_perm(w2, w3, 0x5410),
+                  __byte_perm(w2, w3, 0x7632));
         }
     } else {
-      uint32_t b[NT][2];
-      if constexpr (KV == kWinE4m3) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) b[n][half] = movm_trans(pack_f16x2(x[n][2 * half], x[n][2 * half + 1]));
-      }
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i) {
-        if constexpr (KV == kWinMx) {
-          // The block's weights: w * 2^(e - reference), 0 where that is below
-          // 2^-126. (A NaN exponent is the reference itself, and makes the block
-          // NaN when it is put back in.)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t down = __byte_perm(ref_e[i / 4] - f.ev[half][i / 4], 0u, 0x0444u | ((i % 4) << 12)) >> 1;
-            const float by = __uint_as_float(0x3f800000u - min(down, 127u << 23));
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              b[n][half] = movm_trans(pack_f16x2(x[n][2 * half] * by, x[n][2 * half + 1] * by));
-          }
-        }
         const uint32_t l0 = __byte_perm(f.v[i][0], f.v[i][1], 0x5140), h0 = __byte_perm(f.v[i][0], f.v[i][1], 0x7362);
         const uint32_t l1 = __byte_perm(f.v[i][2], f.v[i][3], 0x5140), h1 = __byte_perm(f.v[i][2], f.v[i][3], 0x7362);
+        uint32_t by0 = 0, by1 = 0;
+        if constexpr (KV == kWinMx) {
+          by0 = exp_pair(f.ev[0][i / 4], f.ev[1][i / 4], i % 4);
+          by1 = exp_pair(f.ev[2][i / 4], f.ev[3][i / 4], i % 4);
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           uint32_t a0, a1, a2, a3;
-          e4m3x4_f16(u ? h0 : l0, a0, a1);
-          e4m3x4_f16(u ? h1 : l1, a2, a3);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) win_mma<true>(o[n][2 * i + u], a0, a1, a2, a3, b[n][0], b[n][1]);
+          if constexpr (KV == kWinMx) {
+            e4m3x4_bf16_by(u ? h0 : l0, by0, a0, a1);
+            e4m3x4_bf16_by(u ? h1 : l1, by1, a2, a3);
+          } else {
+            e4m3x4_f16(u ? h0 : l0, a0, a1);
+            e4m3x4_f16(u ? h1 : l1, a2, a3);
+          }
+          product(2 * i + u, a0, a1, a2, a3);
         }
       }
     }
@@ -632,7 +618,7 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
       float inv = t == 0.f ? 0.f : 1.f / t;
       if (KV == kWinE4m3) inv *= reinterpret_cast<const float*>(a.scales)[a.Hkv + h];
       if (g == 0) {
-        sh.m[warp][r] = m[n][e] - (kF16 ? kWinF16Shift : 0.f);
+        sh.m[warp][r] = m[n][e] - (kF16V ? kWinF16Shift : 0.f);
         sh.l[warp][r] = t;
       }
       if constexpr (KV == kWinBf16) {
@@ -644,11 +630,9 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-          const float by = KV == kWinMx ? inv * e8m0_byte_to_float(ref_e[i / 4], i % 4) : inv;
+        for (int i = 0; i < kBlocks; ++i)
           *reinterpret_cast<float4*>(&sh.o[warp][r][32 * i + 4 * g]) =
-              make_float4(o[n][2 * i][e] * by, o[n][2 * i][e + 2] * by, o[n][2 * i + 1][e] * by, o[n][2 * i + 1][e + 2] * by);
-        }
+              make_float4(o[n][2 * i][e] * inv, o[n][2 * i][e + 2] * inv, o[n][2 * i + 1][e] * inv, o[n][2 * i + 1][e + 2] * inv);
       }
     }
   __syncthreads();
