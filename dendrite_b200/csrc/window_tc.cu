@@ -422,7 +422,9 @@ __global__ void __maxnreg__((WtCfg<D, KV>::kRegs))
     int tiles = 0;             // its tiles so far
     bool ok = true;
     // f16: this thread's row of the item's Q, bf16 as loaded, to f16 in place;
-    // returns the power of two that it was multiplied by.
+    // returns the power of two that it was multiplied by. The sign of the head's
+    // K scale goes into the row, and so does NaN: the maximum is taken before the
+    // scale, and a masked score, -inf, has to stay that.
     auto convert_q = [&]() {
       int up = 0;
       if constexpr (kF16) {
@@ -437,7 +439,9 @@ __global__ void __maxnreg__((WtCfg<D, KV>::kRegs))
           for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
         }
         up = f16_row_shift(top);
-        const float by = __uint_as_float((uint32_t)(127 + up) << 23);
+        float by = __uint_as_float((uint32_t)(127 + up) << 23);
+        const float k_scale = reinterpret_cast<const float*>(a.scales)[it.h];
+        if (!(k_scale >= 0.f)) by = k_scale < 0.f ? -by : k_scale;
 #pragma unroll
         for (int c = 0; c < D / 8; ++c) {
           uint4* at = reinterpret_cast<uint4*>(qx + (c >> 3) * kHalf + (((c & 7) ^ (r & 7)) << 4));
@@ -462,7 +466,7 @@ __global__ void __maxnreg__((WtCfg<D, KV>::kRegs))
       if constexpr (kF16) {
         // Above zero, which would make NaN of the -inf of a masked score (the
         // scores of a row of zeros, whose power of two is the largest, stay zero).
-        scale_log2 = fmaxf(f16_score_scale(a.scale_log2, up) * reinterpret_cast<const float*>(a.scales)[cur.h], FLT_MIN);
+        scale_log2 = fmaxf(f16_score_scale(a.scale_log2, up) * fabsf(reinterpret_cast<const float*>(a.scales)[cur.h]), FLT_MIN);
         v_scale = reinterpret_cast<const float*>(a.scales)[a.Hkv + cur.h];
       }
       const int32_t p = cur.p_lo + tok;

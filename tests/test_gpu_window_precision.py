@@ -137,3 +137,38 @@ def test_mxfp8_nan_exponents(cuda, shape, form, tokens, new):
         bad[rows, h] = True
     assert torch.equal(out.isnan().cpu(), bad)
     assert torch.equal(lse.isnan().cpu(), bad[..., 0])
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("form,tokens,new", FORMS, ids=FORM_IDS)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 4)])
+def test_e4m3_scales_of_either_sign(cuda, shape, form, tokens, new, window, sinks):
+    b = Batch(60 + window, tokens, new, *shape[:3], "e4m3", shape[3], window, sinks)
+    b.scales[0, ::2] *= -1
+    b.scales[1, 1::2] *= -1
+    out, lse = _run(b, form, cuda)
+    check_attention(out, lse, b.attention(), f"{shape} {form} {window}", WEIGHTS["e4m3"])
+
+
+@pytest.mark.parametrize("which", [0], ids=["K"])
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+@pytest.mark.parametrize("form,tokens,new", FORMS + [("decode", [0, 20, 0], [1] * 3), ("many", [5, 0, 300], [40, 7, 260])])
+def test_e4m3_nan_scales(cuda, which, shape, form, tokens, new):
+    """A NaN scale makes its head's rows NaN; rows that see nothing stay zeros, and other heads what they are."""
+    Hq, Hkv, D, grouped = shape
+    b = Batch(61, tokens, new, Hq, Hkv, D, "e4m3", grouped, 100, 4)
+    good, good_lse = _run(b, form, cuda)
+    b.scales[which, 0] = float("nan")
+    out, lse = _run(b, form, cuda)
+    sees = torch.tensor([n - m + i >= 0 for n, m in zip(tokens, new) for i in range(m)])
+    bad = torch.zeros(out.shape[:2], dtype=torch.bool)
+    for h in range(Hq):
+        if (h // (Hq // Hkv) if grouped else h % Hkv) == 0:
+            bad[:, h] = sees
+    bad = bad.to(cuda)
+    assert out[bad].isnan().all() and torch.equal(out[~bad], good[~bad])
+    assert torch.equal(lse[~bad], good_lse[~bad])
+    if which == 0:
+        assert lse[bad].isnan().all()
+    else:
+        assert torch.equal(lse, good_lse)
