@@ -615,8 +615,8 @@ __global__ void __launch_bounds__(kWinWarps * 32, kWinCtas<D, KV, NT>) win_mma_k
 #pragma unroll
       for (int b = 4; b < 32; b <<= 1) t += __shfl_xor_sync(0xffffffffu, t, b);
       const int r = 8 * n + 2 * c + e;
-      float inv = t == 0.f ? 0.f : 1.f / t;
-      if (KV == kWinE4m3) inv *= reinterpret_cast<const float*>(a.scales)[a.Hkv + h];
+      const float v_scale = KV == kWinE4m3 ? reinterpret_cast<const float*>(a.scales)[a.Hkv + h] : 1.f;
+      const float inv = t == 0.f ? 0.f : v_scale * (1.f / t);
       if (g == 0) {
         sh.m[warp][r] = m[n][e] - (kF16V ? kWinF16Shift : 0.f);
         sh.l[warp][r] = t;

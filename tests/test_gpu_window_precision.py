@@ -150,7 +150,7 @@ def test_e4m3_scales_of_either_sign(cuda, shape, form, tokens, new, window, sink
     check_attention(out, lse, b.attention(), f"{shape} {form} {window}", WEIGHTS["e4m3"])
 
 
-@pytest.mark.parametrize("which", [0], ids=["K"])
+@pytest.mark.parametrize("which", [0, 1], ids=["K", "V"])
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
 @pytest.mark.parametrize("form,tokens,new", FORMS + [("decode", [0, 20, 0], [1] * 3), ("many", [5, 0, 300], [40, 7, 260])])
 def test_e4m3_nan_scales(cuda, which, shape, form, tokens, new):
