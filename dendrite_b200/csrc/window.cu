@@ -214,7 +214,10 @@ static int window_attention(const dd_attn_config* cfg, int32_t num_seqs, int32_t
   a.scale_log2 = scale * kLog2e;
   if (cfg->q_dtype == DD_DTYPE_F32 || cfg->kv_dtype == DD_DTYPE_F32) return launch_win_simple(a, st);
   int nsplit = 1;
-  if (q_indptr && win_tc_fits(a) && tc_is_faster(a, max_pages, nsplit)) return launch_win_tc(a, nsplit, st);
+  if (q_indptr && win_tc_fits(a) && tc_is_faster(a, max_pages, nsplit)) {
+    const int rc = launch_win_tc(a, nsplit, st);
+    if (rc != DD_ERR_NOT_AVAILABLE) return rc;
+  }
   return launch_win_mma(a, max_pages, st);
 }
 

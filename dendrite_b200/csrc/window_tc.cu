@@ -1017,7 +1017,7 @@ static cudaError_t launch_win_tc_t(const CUtensorMap& kv, const CUtensorMap& q, 
     cudaFuncAttributes fa;
     e = cudaFuncGetAttributes(&fa, win_tc_kernel<D, KV, kSplit>);
     if (e != cudaSuccess) return e;
-    if (fa.numRegs < Cfg::kRegs) return cudaErrorInvalidConfiguration;
+    if (fa.numRegs < Cfg::kRegs) return cudaErrorLaunchOutOfResources;
   }
   ProfScope ps(kProfTc, st);
   cudaLaunchConfig_t cfg = {};
@@ -1068,6 +1068,7 @@ int win_tc_split(int64_t items, int64_t pages, int sms) {
   return n;
 }
 
+// DD_ERR_NOT_AVAILABLE: not launched, the registers do not hold it.
 int launch_win_tc(const WinArgs& a, int nsplit, cudaStream_t st) {
   CUtensorMap kv, q;
   int rc = make_kv_tensor_map(&kv, a.kv, a.num_pages, a.Hkv, a.D, a.kv_dtype == DD_DTYPE_BF16 ? 2 : 1, 0);
@@ -1077,6 +1078,10 @@ int launch_win_tc(const WinArgs& a, int nsplit, cudaStream_t st) {
   const auto launch = a.D == 64 ? (nsplit > 1 ? launch_win_tc_kv<64, true> : launch_win_tc_kv<64, false>)
                                 : (nsplit > 1 ? launch_win_tc_kv<128, true> : launch_win_tc_kv<128, false>);
   const cudaError_t e = launch(kv, q, a, units, nsplit, st);
+  if (e == cudaErrorLaunchOutOfResources) {
+    cudaGetLastError();
+    return DD_ERR_NOT_AVAILABLE;
+  }
   if (e != cudaSuccess) return fail(DD_ERR_CUDA, std::string("window attention launch: ") + cudaGetErrorString(e));
   return DD_OK;
 }
