@@ -39,6 +39,9 @@ prompts in flight or tokens to be checked) goes in through
   FP8 pools) and returns the causal attention, windowed or full;
 
 and ``read_tokens`` takes token ranges back out, dequantised.
+
+A page id that is not in the pool stops no kernel: it is skipped and noted on
+the device, and ``check()`` raises for it (after a step, or every few).
 """
 from __future__ import annotations
 
@@ -94,6 +97,7 @@ class PagedKVCache:
         self._ws: dict = {}
         self._page_ids = self._slots = None
         self._step = self._chunks = None  # device tables of the step / of the chunks
+        self._status = torch.zeros(2, dtype=torch.int32, device=self.device)  # of every call, until check()
 
     # -- per step ---------------------------------------------------------
     def _only_grew(self, indptr, block_ids) -> bool:
@@ -172,12 +176,12 @@ class PagedKVCache:
             raise _lib.InvalidArgument("begin_step first")
         self._check_rows(q, k, v, len(self._page_ids))
         append_kv_batch(self.cfg, self.pools[layer], self.scales[layer], self._page_ids, self._slots,
-                        k.contiguous(), v.contiguous())
+                        k.contiguous(), v.contiguous(), status=self._status)
         q = q.to(torch.bfloat16).contiguous()
         if self.windows[layer]:
             ip, ids, ntok, longest = self._step
             out, _ = decode_paged_window(self.cfg, q, self.pools[layer], ip, ids, ntok, *self.windows[layer],
-                                         max_pages=longest, kv_scales=self.scales[layer])
+                                         max_pages=longest, kv_scales=self.scales[layer], status=self._status)
             return out
         ws = _alloc_ws(self.plan.info().workspace_bytes, self.device, self._ws)
         out, _ = cascade_decode(self.cfg, self.plan, q, self.pools[layer], self.scales[layer],
@@ -203,7 +207,7 @@ class PagedKVCache:
         page_ids = torch.from_numpy(tbl[pos // PAGE_SIZE].astype(np.int32)).to(self.device)
         slots = torch.from_numpy((pos % PAGE_SIZE).astype(np.int32)).to(self.device)
         append_kv_batch(self.cfg, self.pools[layer], self.scales[layer], page_ids, slots,
-                        k.contiguous(), v.contiguous())
+                        k.contiguous(), v.contiguous(), status=self._status)
         plan = CascadePlan.prefill(self.cfg, [0, len(tbl)], tbl, [prefix_len], [S])
         plan.upload(self.device)
         out, _ = cascade_decode(self.cfg, plan, q.to(torch.bfloat16).contiguous(), self.pools[layer],
@@ -241,10 +245,12 @@ class PagedKVCache:
         ip, ids, ntok, longest, borders, rows = tables
         if not q.shape[0] == k.shape[0] == v.shape[0] >= rows:
             raise _lib.InvalidArgument(f"q, k and v must have the batch's {rows} rows")
-        append_kv_paged(self.cfg, self.pools[layer], self.scales[layer], borders, ip, ids, ntok, k, v)
+        append_kv_paged(self.cfg, self.pools[layer], self.scales[layer], borders, ip, ids, ntok, k, v,
+                        status=self._status)
         window, sinks = self.windows[layer] or (0, 0)
         out, _ = prefill_paged_window(self.cfg, q.to(torch.bfloat16), self.pools[layer], borders, ip, ids, ntok,
-                                      window, sinks, max_pages=longest, kv_scales=self.scales[layer])
+                                      window, sinks, max_pages=longest, kv_scales=self.scales[layer],
+                                      status=self._status)
         return out
 
     def read_tokens(self, layer: int, indptr, block_ids, first, count, out_dtype=torch.bfloat16):
@@ -260,4 +266,20 @@ class PagedKVCache:
         ip, pages, start, _ = self._device_tables(indptr, ids, first)
         rows = np.concatenate([[0], np.cumsum(count, dtype=np.int64)]).astype(np.int32)
         return gather_kv_paged(self.cfg, self.pools[layer], self.scales[layer], torch.from_numpy(rows).to(self.device),
-                               start, ip, pages, int(rows[-1]), out_dtype)
+                               start, ip, pages, int(rows[-1]), out_dtype, status=self._status)
+
+    # -- what went wrong on the device ----------------------------------------
+    def check(self) -> None:
+        """Raise if an append, a windowed attention or a read-back since the last
+        check met a page outside the pool or the table (it skipped the page, or
+        read zeros), or gave up a wait. Waits for the current stream; a page
+        that the engine gave back one step too early is found here."""
+        code, where = self._status.tolist()
+        if not code:
+            return
+        self._status.zero_()
+        if code == 1:
+            raise _lib.InvalidArgument("a page outside the pool, or a missing one, was skipped "
+                                       f"(the page, or the row that it was for: {where & 0xffffffff})")
+        raise _lib.CudaError(f"a kernel gave up a wait (status {code}, {where & 0xffffffff}): its outputs are not valid")
+

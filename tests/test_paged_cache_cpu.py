@@ -99,3 +99,43 @@ def test_a_prompt_outside_its_table(windows, table, prefix):
     """Position -1 would be the last slot of the table's last page."""
     with pytest.raises(dd.InvalidArgument, match="fit together"):
         _cache(windows).layer_prefill(0, _rows(2, HQ), _rows(2, HKV), _rows(2, HKV), table, prefix)
+
+
+def test_check_raises_once():
+    cache = _cache([(20, 2)])
+    cache.check()
+    for status, error in (([1, -2], dd.InvalidArgument), ([2, 0], dd.CudaError)):
+        cache._status[:] = torch.tensor(status, dtype=torch.int32)
+        with pytest.raises(error):
+            cache.check()
+        cache.check()
+
+
+def test_every_call_reports_to_the_cache(monkeypatch):
+    import dendrite_b200.paged_cache as pc
+
+    cache, seen = _cache([(20, 2), None]), []
+
+    def call(name, result):
+        def fake(*args, status=None, **kw):
+            assert status is cache._status, name
+            seen.append(name)
+            return result
+        monkeypatch.setattr(pc, name, fake)
+
+    out = _rows(1, HQ)
+    for name, result in (("append_kv_batch", None), ("append_kv_paged", None), ("decode_paged_window", (out, None)),
+                         ("prefill_paged_window", (out, None)), ("gather_kv_paged", (out, out))):
+        call(name, result)
+    monkeypatch.setattr(pc, "cascade_decode", lambda *args, **kw: (out, None))
+    monkeypatch.setattr(dd.CascadePlan, "upload", lambda plan, device=None, stream=None: None)
+    qkv = (_rows(1, HQ), _rows(1, HKV), _rows(1, HKV))
+    cache.begin_step([0, 1], [3], [4])
+    cache.begin_chunks([0, 1], [3], [6], [1])
+    for layer in (0, 1):
+        cache.layer_step(layer, *qkv)
+        cache.layer_chunk(layer, *qkv)
+        cache.layer_prefill(layer, *qkv, [3], 6)
+        cache.read_tokens(layer, [0, 1], [3], [0], [7])
+    assert sorted(set(seen)) == ["append_kv_batch", "append_kv_paged", "decode_paged_window", "gather_kv_paged",
+                                 "prefill_paged_window"] and len(seen) == 7 + 5
