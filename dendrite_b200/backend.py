@@ -20,6 +20,10 @@ over pages: it stores the new tokens' K/V in the block table's pages and runs
 a causal plan (``CascadePlan.prefill``) in which new token i sees the
 sequence's tokens up to its own position.
 
+``AttentionConfig.sliding_window``, which the reference declares and does not
+read, is honoured: a token then attends to the last ``sliding_window`` tokens,
+itself among them, by the window kernels over the same pages.
+
 PyTorch is used only for device memory and the current CUDA stream; all
 arithmetic runs in the CUDA kernels of ``libdendrite_b200.so``.
 """
@@ -35,6 +39,7 @@ import torch
 from . import _lib
 from ._lib import (DTYPE_BF16, DTYPE_E4M3, DTYPE_F32, DTYPE_MXFP8, GQA_GROUPED, GQA_TILED,
                    AttnConfig, NotAvailable, PlanInfo, PlanOptions, QuantConfig, check, lib)
+from .paged_window import decode_paged_window, prefill_paged_window
 
 PAGE_SIZE = 16                 # flashinfer/mod.rs:14
 MAX_SEQ_LEN = None             # no compile-time cap (flashinfer/mod.rs:17 capped at 131072)
@@ -414,6 +419,23 @@ class B200Backend:
         return make_config(config.num_heads, config.num_kv_heads, config.head_dim, self.num_pages,
                            kvd, qd, self.gqa_map, config.scale)
 
+    def _window(self, config: AttentionConfig, block_tables) -> int:
+        """The window of a call, 0 for full attention. Nothing but the plan of full attention looks
+        at the block tables on the host, so they are checked here."""
+        if config.sliding_window is None:
+            return 0
+        if config.sliding_window < 1:
+            raise _lib.InvalidArgument("sliding_window must be >= 1")
+        for t in block_tables:
+            if t.num_tokens() > t.num_blocks() * PAGE_SIZE:
+                raise _lib.InvalidArgument("num_tokens exceeds its block table")
+            if any(not 0 <= b < self.num_pages for b in t.blocks()):
+                raise _lib.InvalidArgument("invalid block id")
+        return min(config.sliding_window, (1 << 31) - 1)
+
+    def _ints(self, values) -> torch.Tensor:
+        return torch.tensor(values, dtype=torch.int32).to(self.device)
+
     def append_kv(self, key: torch.Tensor, value: torch.Tensor, block_table: BlockTable,
                   position: int) -> None:
         """backend.rs:285-301: store [1, Hkv, t, D] K/V in block_table[position // 16]."""
@@ -450,6 +472,7 @@ class B200Backend:
             raise _lib.InvalidArgument("block_table must count the prefill tokens (num_tokens >= seq_len)")
         if block_table.num_blocks() * PAGE_SIZE < prefix + S:
             raise _lib.InvalidArgument("block_table has too few blocks for the prefill tokens")
+        window = self._window(config, [block_table])
         if S == 0:
             return query.clone()
         pos = torch.arange(prefix, prefix + S)
@@ -472,6 +495,13 @@ class B200Backend:
         qd = torch.float32 if q.dtype == torch.float32 else torch.bfloat16
         q = q.to(qd).contiguous()
         cfg = self._cfg(config, qd)
+        if window:
+            kv, sc = self._kv()
+            n = block_table.num_blocks()
+            out, _ = prefill_paged_window(cfg, q, kv, self._ints([0, S]), self._ints([0, n]),
+                                          self._ints(block_table.blocks()), self._ints([prefix + S]), window,
+                                          max_pages=n, kv_scales=sc)
+            return out.transpose(0, 1).reshape(query.shape).to(query.dtype)
         plan = CascadePlan.prefill(cfg, [0, block_table.num_blocks()], block_table.blocks(), [prefix], [S])
         plan.upload(self.device)
         kv, sc = self._kv()
@@ -488,15 +518,23 @@ class B200Backend:
         """backend.rs:267-283, as one cascade launch over the batch."""
         if not queries:
             return []
+        window = self._window(config, block_tables)
         q = torch.stack([x.reshape(config.num_heads, config.head_dim) for x in queries])
         qd = torch.float32 if q.dtype == torch.float32 else torch.bfloat16
         q = q.to(qd).contiguous()
         cfg = self._cfg(config, qd)
-        plan = CascadePlan.from_tables(cfg, block_tables)
-        plan.upload(self.device)
         kv, sc = self._kv()
-        ws = _alloc_ws(plan.info().workspace_bytes, self.device, self._ws)
-        out, _ = cascade_decode(cfg, plan, q, kv, sc, workspace=ws)
+        if window:
+            lens = [t.num_blocks() for t in block_tables]
+            indptr = np.cumsum([0] + lens)
+            out, _ = decode_paged_window(cfg, q, kv, self._ints(indptr), self._ints([b for t in block_tables for b in t.blocks()]),
+                                         self._ints([t.num_tokens() for t in block_tables]), window,
+                                         max_pages=max(lens, default=0), kv_scales=sc)
+        else:
+            plan = CascadePlan.from_tables(cfg, block_tables)
+            plan.upload(self.device)
+            ws = _alloc_ws(plan.info().workspace_bytes, self.device, self._ws)
+            out, _ = cascade_decode(cfg, plan, q, kv, sc, workspace=ws)
         return [out[i].reshape(queries[i].shape).to(queries[i].dtype) for i in range(len(queries))]
 
     def decode(self, query: torch.Tensor, block_table: BlockTable,

@@ -32,6 +32,8 @@ def _fail(msg: str):
 
 def _check_pool(cfg: AttnConfig, kv_pages, kv_scales) -> None:
     kvd = cfg.kv_dtype
+    if kv_pages is None:
+        _fail("kv_pages is None")
     if kv_pages.dtype not in _POOL.get(kvd, ()) or not kv_pages.is_contiguous() or \
             kv_pages.shape != (cfg.num_pages, 2, cfg.num_kv_heads, cfg.page_size, cfg.head_dim):
         _fail("kv_pages must be a dense [num_pages][2][Hkv][16][D] pool of the config's kv_dtype")
