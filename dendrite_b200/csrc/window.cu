@@ -137,28 +137,36 @@ int launch_win_simple(const WinArgs& a, cudaStream_t st) {
 
 // Chunks: which of the two tensor-core kernels, and in how many CTAs the tcgen05
 // one splits an item. Both walk the visible pages of every KV head, the streaming
-// kernel once for 16 rows at about 1.5 ns (bf16; FP8 1.1) a page for the whole GPU
-// (two pages' bytes from L2, or HBM), the tcgen05 kernel once for up to 256 rows
-// at 1.9 us (MXFP8 2.15) for 8 pages on one SM, and 8 or 9 us more where shares
-// are joined. Measured around the border (streaming, tcgen05; us), windows of
-// 1024, 2048, 4096 tokens: 64 sequences x 4 new tokens, bf16, 4 heads a group 63,
-// 79; x 8 110, 79; E4M3, 8 heads a group x 2 72, 138; x 4 167, 138; MXFP8, 4 heads
-// a group x 4 152, 287; one sequence x 64, bf16, 18, 24; x 128 26, 24; without a
-// window, 16,000 tokens, x 8 41, 37; x 32 75, 40; x 256 556, 86.
+// kernel once for 16 rows (or a sequence's fewer), at a time for the whole GPU
+// that goes by the page's bytes and their unpacking, the tcgen05 kernel once for up
+// to 256, 8 pages after 8 on one SM a CTA, items in waves, with more to set up and
+// shares to join. The constants are fitted to 1152 measured pairs (1 to 64
+// sequences x 2 to 256 new tokens, windows of 16 to 4096 and none over 8000 tokens,
+// 1, 4 and 8 heads a group, head dims 64 and 128): the choice is more than 1.2 times
+// the better one in 2 of them, and in 4 of 400 ragged batches drawn from the same
+// ranges. Around the border (streaming, tcgen05; us), head dim 128: bf16, 4 heads a
+// group, window 1024, 16 sequences x 8 new tokens 28.1, 29.4; x 16 54.8, 29.3; 64 x 4
+// 65.3, 93.0; x 8 113.9, 92.8; window 16, 64 x 4 19.5, 23.4; x 8 32.4, 23.6; no
+// window, 1 x 8 26.7, 29.2; x 32 43.7, 30.9; E4M3, 8 heads, window 4096, 16 x 4 59.7,
+// 68.7; x 8 114.2, 68.5; MXFP8, 4 heads, window 1024, 16 x 8 30.6, 32.3; x 16 56.9,
+// 32.3; head dim 64: bf16 16 x 8 20.0, 25.4; x 16 29.8, 25.4; E4M3 16 x 4 42.9, 59.4;
+// x 8 72.9, 59.7.
 static bool tc_is_faster(const WinArgs& a, int max_pages, int& nsplit) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const int64_t rows = (int64_t)a.num_rows * a.g, tokens = a.num_rows / a.num_seqs;
+  const int64_t tokens = a.num_rows / a.num_seqs;
   int64_t pages = max_pages > 0 ? max_pages : 256;
   if (a.window > 0) pages = std::min(pages, ((int64_t)a.window + a.sinks + tokens) / kPageSize + 2);
-  const int64_t tiles16 = std::max<int64_t>(a.num_seqs, (rows + 15) / 16) * a.Hkv;
-  const int64_t items = std::max<int64_t>(a.num_seqs, (rows + 255) / 256) * a.Hkv;
+  const int64_t tiles16 = win_tiles_expected(a, 16) * a.Hkv;
+  const int64_t items = win_tiles_expected(a, 2 * (128 / a.g) * a.g) * a.Hkv;
   nsplit = win_tc_split(items, pages, sms);
   const int64_t tiles = ((pages + 7) / 8 + nsplit - 1) / nsplit;  // of a CTA
-  const int64_t tile_ns = a.kv_dtype == DD_DTYPE_MXFP8 ? 2150 : 1900;
-  const int64_t join_ns = nsplit == 1 ? 0 : tokens * a.g > 128 ? 9000 : 8000;
-  const int64_t stream_ns = 7000 + tiles16 * pages * (a.kv_dtype == DD_DTYPE_BF16 ? 15 : 11) / 10;
-  const int64_t tc_ns = (items * nsplit + sms - 1) / sms * (tiles * tile_ns + 4000) + join_ns;
+  // A page's time in hundredths of a nanosecond.
+  const int64_t page = a.kv_dtype == DD_DTYPE_BF16 ? (a.D == 64 ? 55 : 110) : a.kv_dtype == DD_DTYPE_E4M3 ? (a.D == 64 ? 45 : 80)
+                                                                                                       : (a.D == 64 ? 75 : 100);
+  const int64_t stream_ns = 5200 + tiles16 * (1500 + pages * page) / 100;
+  const int64_t join_ns = nsplit == 1 ? 0 : tokens * a.g > 128 ? 10000 : 4000;
+  const int64_t tc_ns = 7500 + (items * nsplit + sms - 1) / sms * (2300 + tiles * 1700) + join_ns;
   return tc_ns < stream_ns;
 }
 

@@ -143,6 +143,14 @@ __device__ __forceinline__ void win_tile(const WinArgs& a, int g, int R, int64_t
   tile = (int32_t)max(t - base(lo), (int64_t)-1);
 }
 
+// Tiles of R rows that a chunk call's sequences fill, as far as the host knows:
+// all of one length where that divides, else each with half a tile over.
+inline int64_t win_tiles_expected(const WinArgs& a, int R) {
+  const int64_t seqs = a.num_seqs, rows = (int64_t)a.num_rows * a.g;
+  if (a.num_rows % a.num_seqs == 0) return seqs * ((rows / seqs + R - 1) / R);
+  return seqs > rows / R + seqs / 2 ? seqs : rows / R + seqs / 2;
+}
+
 // Another CTA's shared memory: reads at the place that `addr` is in this one's.
 __device__ __forceinline__ float cluster_ld(uint32_t addr, uint32_t rank) {
   uint32_t r;

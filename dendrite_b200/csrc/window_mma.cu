@@ -729,8 +729,7 @@ static int launch_win_mma_t(const WinArgs& a, int max_pages, int sms, cudaStream
   constexpr int R = 8 * NT;
   const int64_t tiles = a.row_indptr ? a.num_seqs + (int64_t)a.num_rows * a.g / R
                                      : (int64_t)a.num_seqs * ((a.g + R - 1) / R);
-  // Tiles that have rows, as far as it is known here.
-  const int64_t full = a.row_indptr ? std::max<int64_t>(a.num_seqs, (int64_t)a.num_rows * a.g / R) : tiles;
+  const int64_t full = a.row_indptr ? win_tiles_expected(a, R) : tiles;  // tiles that have rows
   int64_t pages = max_pages > 0 ? max_pages : INT64_MAX;
   if (a.window > 0) pages = std::min(pages, ((int64_t)a.window + a.sinks) / kPageSize + 2);
   const int nsplit = win_split(full * a.Hkv, (int64_t)sms * kWinCtas<D, KV, NT>, pages);

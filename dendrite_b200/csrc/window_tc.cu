@@ -1061,7 +1061,7 @@ bool win_tc_fits(const WinArgs& a) {
 // the GPU idle, as long as a share is four tiles or more. Eight CTAs, which take
 // an SM each, have to fit one group of SMs: such clusters fill some three
 // quarters of the GPU. (16,000 tokens, window 0, 8 heads, bf16, 32 / 256 new
-// ones: 40 / 85 us, against 75 / 556 of the streaming kernel.)
+// ones: 45 / 94 us, against 76 / 557 of the streaming kernel.)
 int win_tc_split(int64_t items, int64_t pages, int sms) {
   int n = 1;
   while (n < kWtSplit && items * n * 2 * (n == 4 ? 4 : 3) <= sms * 3 && pages >= 4 * kTcPagesPerTile * 2 * n) n *= 2;

@@ -5,22 +5,20 @@ import pytest
 import torch
 
 from tests.test_gpu_window import Dev
+from tests.test_gpu_window_chunk_kernel import WEIGHTS, chunk_kernel
 from tests.window_ref import HALF, Batch, check_attention
 
 pytestmark = pytest.mark.gpu
 
-# (form, tokens, new): one token each; a few; chunks for the tcgen05 kernel; a chunk whose tiles are shared out.
+# (form, tokens, new): one token each; a few; chunks for the tcgen05 kernel; without a window, one whose tiles are shared out.
 FORMS = [("decode", [90, 300, 17, 700], [1] * 4), ("few", [90, 300, 17, 700], [3, 2, 5, 1]),
-         ("many", [90, 300, 700], [33, 140, 260]), ("split", [2500], [130])]
+         ("many", [90, 400, 1100], [33, 240, 900]), ("split", [9000], [900])]
 FORM_IDS = [f[0] for f in FORMS]
-# What a weight is off by: two bf16 terms, both cut off after 8 bits (what the first leaves is below
-# 2^-7 of the weight, what the second leaves below 2^-7 of that); one f16 term, rounded.
-WEIGHTS = {"bf16": 2.0 ** -14, "mxfp8": 2.0 ** -14, "e4m3": 2.0 ** -11}
-
-
 def _run(b, form, dev, **kw):
     d = Dev(b, dev)
-    return (d.decode if form == "decode" else d.prefill)(**kw)
+    if form == "decode":
+        return d.decode(**kw)
+    return chunk_kernel(d.prefill) if form in ("many", "split") and b.D <= 128 else d.prefill(**kw)
 
 
 def _check(got, lse, want, weights, what):
@@ -152,7 +150,7 @@ def test_e4m3_scales_of_either_sign(cuda, shape, form, tokens, new, window, sink
 
 @pytest.mark.parametrize("which", [0, 1], ids=["K", "V"])
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
-@pytest.mark.parametrize("form,tokens,new", FORMS + [("decode", [0, 20, 0], [1] * 3), ("many", [5, 0, 300], [40, 7, 260])])
+@pytest.mark.parametrize("form,tokens,new", FORMS + [("decode", [0, 20, 0], [1] * 3), ("many", [5, 0, 1000], [40, 7, 960])])
 def test_e4m3_nan_scales(cuda, which, shape, form, tokens, new):
     """A NaN scale makes its head's rows NaN; rows that see nothing stay zeros, and other heads what they are."""
     Hq, Hkv, D, grouped = shape
