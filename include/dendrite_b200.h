@@ -324,7 +324,9 @@ int dd_decode_paged_static_status(dd_stream_t stream, uint32_t* code, uint32_t* 
  * status[0] = 2: a bounded wait ran out and the outputs are not valid.
  * Tokens that some new token of a sequence sees must be finite for all of
  * that call's rows of the sequence to be: a row whose own window excludes
- * them may still multiply them by a weight of zero.
+ * them may still multiply them by a weight of zero. kv_scales of E4M3 pages may
+ * have either sign; a NaN makes its head's rows NaN. Weights keep 16 bits (bf16
+ * and MXFP8 pages) or 11 (E4M3), whichever kernel takes the call.
  *
  * q: rows of [num_qo_heads][head_dim], q_stride elements from row to row
  * (>= num_qo_heads * head_dim, a multiple of 16 bytes, so that the queries of
