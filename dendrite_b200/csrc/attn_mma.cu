@@ -854,6 +854,8 @@ int mma_row_tile() { return kMmaRows; }
 // counter in the workspace header must be zero (the caller resets the header).
 int launch_attn_mma(const AttnArgs& a, int64_t num_pages, cudaStream_t st, bool after_tc) {
   if (a.num_items <= 0) return DD_OK;
+  if (!mma_supported(a.D, a.kv_dtype))
+    return fail(DD_ERR_NOT_AVAILABLE, "streaming tensor-core kernel: bf16 KV at head_dim 64 / 128, FP8 KV at 128");
   CUtensorMap map;
   const int eb = a.kv_dtype == DD_DTYPE_BF16 ? 2 : 1;
   int rc = make_kv_tensor_map(&map, a.kv, num_pages, a.Hkv, a.D, eb,

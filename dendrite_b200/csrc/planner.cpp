@@ -75,9 +75,10 @@ extern "C" int dd_tc_available(void);  // attn_tc.cu
 
 namespace dd {
 
+bool mma_supported(int D, int kv_dtype);  // attn_mma.cu
+
 static int kind_for(const dd_attn_config& c, const dd_plan_options& o, int64_t rows) {
-  if (c.kv_dtype == DD_DTYPE_F32 || c.q_dtype != DD_DTYPE_BF16 || c.head_dim > 128)
-    return kItemSimple;
+  if (c.q_dtype != DD_DTYPE_BF16 || !mma_supported(c.head_dim, c.kv_dtype)) return kItemSimple;
   const bool tc = o.use_tensor_cores && c.head_dim == 128 && dd_tc_available();
   if (tc && o.cta_pairs && rows > 256 && c.kv_dtype == DD_DTYPE_BF16) return kItemTc2;
   if (tc && rows >= 128) return kItemTc;
