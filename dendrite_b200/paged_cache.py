@@ -57,6 +57,16 @@ from .paged_window import (append_kv_paged, decode_paged_window, gather_kv_paged
 _KV = {"bf16": _lib.DTYPE_BF16, "e4m3": _lib.DTYPE_E4M3, "mxfp8": _lib.DTYPE_MXFP8}
 
 
+def _rows_in_place(t: torch.Tensor) -> torch.Tensor:
+    """[rows, heads, dim] as the window kernels take it: itself where its heads are dense and its rows
+    lie on 16 bytes (part of a wider projection), else a dense copy."""
+    width = t.shape[1] * t.shape[2]
+    if t.data_ptr() % 16 == 0 and t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == t.shape[2]) and \
+            (t.shape[0] <= 1 or (t.stride(0) >= width and t.stride(0) * t.element_size() % 16 == 0)):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 class PagedKVCache:
     """Page pools of `num_layers` layers ([num_pages][2][Hkv][16][D] each) and
     the step's cascade plan, shared by the layers."""
@@ -177,14 +187,14 @@ class PagedKVCache:
         self._check_rows(q, k, v, len(self._page_ids))
         append_kv_batch(self.cfg, self.pools[layer], self.scales[layer], self._page_ids, self._slots,
                         k.contiguous(), v.contiguous(), status=self._status)
-        q = q.to(torch.bfloat16).contiguous()
+        q = _rows_in_place(q.to(torch.bfloat16))
         if self.windows[layer]:
             ip, ids, ntok, longest = self._step
             out, _ = decode_paged_window(self.cfg, q, self.pools[layer], ip, ids, ntok, *self.windows[layer],
                                          max_pages=longest, kv_scales=self.scales[layer], status=self._status)
             return out
         ws = _alloc_ws(self.plan.info().workspace_bytes, self.device, self._ws)
-        out, _ = cascade_decode(self.cfg, self.plan, q, self.pools[layer], self.scales[layer],
+        out, _ = cascade_decode(self.cfg, self.plan, q.contiguous(), self.pools[layer], self.scales[layer],
                                 workspace=ws)
         return out
 
@@ -210,7 +220,7 @@ class PagedKVCache:
                         k.contiguous(), v.contiguous(), status=self._status)
         plan = CascadePlan.prefill(self.cfg, [0, len(tbl)], tbl, [prefix_len], [S])
         plan.upload(self.device)
-        out, _ = cascade_decode(self.cfg, plan, q.to(torch.bfloat16).contiguous(), self.pools[layer],
+        out, _ = cascade_decode(self.cfg, plan, _rows_in_place(q.to(torch.bfloat16)).contiguous(), self.pools[layer],
                                 self.scales[layer])
         return out
 
@@ -245,11 +255,11 @@ class PagedKVCache:
         ip, ids, ntok, longest, borders, rows = tables
         if not q.shape[0] == k.shape[0] == v.shape[0] >= rows:
             raise _lib.InvalidArgument(f"q, k and v must have the batch's {rows} rows")
-        append_kv_paged(self.cfg, self.pools[layer], self.scales[layer], borders, ip, ids, ntok, k, v,
-                        status=self._status)
+        append_kv_paged(self.cfg, self.pools[layer], self.scales[layer], borders, ip, ids, ntok, _rows_in_place(k),
+                        _rows_in_place(v), status=self._status)
         window, sinks = self.windows[layer] or (0, 0)
-        out, _ = prefill_paged_window(self.cfg, q.to(torch.bfloat16), self.pools[layer], borders, ip, ids, ntok,
-                                      window, sinks, max_pages=longest, kv_scales=self.scales[layer],
+        out, _ = prefill_paged_window(self.cfg, _rows_in_place(q.to(torch.bfloat16)), self.pools[layer], borders, ip,
+                                      ids, ntok, window, sinks, max_pages=longest, kv_scales=self.scales[layer],
                                       status=self._status)
         return out
 
