@@ -185,14 +185,16 @@ class PagedKVCache:
         if self._page_ids is None:
             raise _lib.InvalidArgument("begin_step first")
         self._check_rows(q, k, v, len(self._page_ids))
-        append_kv_batch(self.cfg, self.pools[layer], self.scales[layer], self._page_ids, self._slots,
-                        k.contiguous(), v.contiguous(), status=self._status)
         q = _rows_in_place(q.to(torch.bfloat16))
         if self.windows[layer]:
             ip, ids, ntok, longest = self._step
+            append_kv_paged(self.cfg, self.pools[layer], self.scales[layer], None, ip, ids, ntok, _rows_in_place(k),
+                            _rows_in_place(v), status=self._status)
             out, _ = decode_paged_window(self.cfg, q, self.pools[layer], ip, ids, ntok, *self.windows[layer],
                                          max_pages=longest, kv_scales=self.scales[layer], status=self._status)
             return out
+        append_kv_batch(self.cfg, self.pools[layer], self.scales[layer], self._page_ids, self._slots,
+                        k.contiguous(), v.contiguous(), status=self._status)
         ws = _alloc_ws(self.plan.info().workspace_bytes, self.device, self._ws)
         out, _ = cascade_decode(self.cfg, self.plan, q.contiguous(), self.pools[layer], self.scales[layer],
                                 workspace=ws)
