@@ -1,5 +1,6 @@
 // CUDA-core partial attention over one work item: the path for f32 KV pages
-// (TinyLlama-shaped parity config), head_dim 256, and f32 queries.
+// (TinyLlama-shaped parity config), head_dim 256, FP8 KV pages at head_dim 64,
+// and f32 queries.
 //
 // Per page it stages K and V (dequantized to f32) in shared memory, computes
 // the scaled scores of every row, does the online-softmax update and

@@ -1,4 +1,4 @@
-"""FP8 pages at head dim 64 through the plans, the paged cache and the backend, against 64 bits."""
+"""FP8 pages at head dims 64 and 256 through the plans, paged decode and the backend, against 64 bits."""
 import numpy as np
 import pytest
 import torch
@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "mxfp8"])
-@pytest.mark.parametrize("shape", [(8, 2, 64, True), (32, 4, 64, False)], ids=str)
+@pytest.mark.parametrize("shape", [(8, 2, 64, True), (32, 4, 64, False), (6, 3, 256, True)], ids=str)
 @pytest.mark.parametrize("form", ["decode", "prefill", "flat"])
 def test_plans(cuda, fmt, shape, form):
     tokens = [300, 77, 16, 1]
@@ -25,7 +25,7 @@ def test_plans(cuda, fmt, shape, form):
             dd.CascadePlan.prefill(d.cfg, b.indptr, np.array(b.ids), [n - m for n, m in zip(tokens, new)], new)
         out, lse = dd.cascade_decode(d.cfg, plan, d.q, d.pool, d.scales)
     # E4M3: code * scale is rounded to bf16, so V is off by 2^-8 and so, times reach, are the scores
-    # (64 2^-24 2^10 = 2^-8); MXFP8's code * 2^e is exact. The weights stay in f32.
+    # (D 2^-24 2^10 >= 2^-8); MXFP8's code * 2^e is exact. The weights stay in f32.
     want, weights = b.attention(), 2.0 ** -14
     if fmt == "e4m3":
         weights, want = weights + 2.0 ** -8, (*want[:3], want[3] * 2.0 ** 10, want[4])
